@@ -20,6 +20,7 @@
 #ifndef MT_SCHED_H
 #define MT_SCHED_H
 #include <stddef.h>
+#include <stdint.h>
 
 #ifdef __cplusplus
 extern "C" {
@@ -125,6 +126,33 @@ int mt_sched_add_lengths(MT_POOL_ARGS, const int* slots, const int* tokens, int 
 int mt_sched_decode_abort(MT_POOL_ARGS, const int* slots, int b, const int* new_page);
 
 #undef MT_POOL_ARGS
+
+/* A step's block tables, slot map, positions and token offsets from the
+ * requests' lengths, without a pool state: request r holds lengths[r] tokens
+ * and gets tokens[r] more (tokens null: one each), whose pages come in request
+ * order from the flat list pages[page_count]. With old = ceil(lengths[r] /
+ * page_size) and new = ceil((lengths[r] + tokens[r]) / page_size), row r of
+ * table [b, columns] (in and out) gets its new - old pages in columns [old,
+ * new); a row that starts with this step (length 0) also gets -1 behind them,
+ * the rest of a row is left as it was. The new tokens lie request after request
+ * from cu_tokens[r] on (cu_tokens [b + 1] = exclusive sums of tokens, at most
+ * `rows`): for token i of request r, at p = lengths[r] + i, slots[cu_tokens[r] +
+ * i] = page * page_size + p % page_size (64 bits; what mt_paged_append_slots of
+ * mt_shared.h takes) and positions[..] = (float)(prefix_tokens + p), the place behind
+ * a prefix that every request shares (0 without one; what mt_embed_tokens
+ * takes). slots and positions have `rows` entries: tokens past them are
+ * dropped, slots behind the last token are -1 and positions there are left. A
+ * token has slot -1 where its column is past the table, its table entry is
+ * negative, or the list is exhausted (whose table entries are -1 as well). A request of negative length is
+ * left out: it takes no token and no page, and its row stays. Negative tokens
+ * count as none. lengths, tokens and pages are read on the device and may hold
+ * anything. 1 <= b <= 65535; page_size 8, 16 or 32; page_count 0 needs no list. One launch on the
+ * calling thread's default stream; nothing is allocated. Replaces, for several tokens per request, the host
+ * tables of reference PagedDecodeBatch.prepare (minitorch/paged_decode.py:40-54) and
+ * PagedKVCache.prepare_append (minitorch/paged_kv_cache.py:171-189). */
+int mt_sched_batch_tables(int* table, int64_t* slots, float* positions, int* cu_tokens, const int* lengths,
+                          const int* tokens, const int* pages, int b, int rows, int page_count, int columns,
+                          int page_size, int prefix_tokens);
 
 #ifdef __cplusplus
 }

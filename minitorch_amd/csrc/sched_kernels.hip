@@ -19,6 +19,7 @@
 // The state blob layout is computed by pool_layout() and exported through
 // mt_pool_layout() so the host can address the slab table and slot rows.
 #include "mt_device.h"
+#include <algorithm>
 #include <climits>
 
 namespace {
@@ -630,6 +631,154 @@ __global__ __launch_bounds__(kThreads) void decode_abort_kernel(Pool p, const in
   }
 }
 
+// ---------------------------------------------------------------------------
+// Block tables and slot map of a step, from the requests' lengths
+// (mt_sched_batch_tables). A workgroup owns a chunk of kChunk requests and one of
+// `slices` shares of that chunk's tokens, pages and started rows: it sums what the
+// requests before its chunk take (a strided reduction, nothing for the first),
+// scans its own in LDS, and finds the request of each token or page by bisection
+// there. One launch, no scratch memory, no order between workgroups: an entry of
+// the table that is read (a started page, held before the step) is never one that
+// is written. Bound by latency (lengths, then pages, then stores) up to some ten
+// thousand tokens, by its stores beyond.
+constexpr int kChunk = 256;
+constexpr int kTableThreads = 256;
+
+struct TableArgs {
+  int* table;
+  int64_t* slots;
+  float* positions;
+  int* cu_tokens;
+  const int* lengths;
+  const int* tokens;
+  const int* pages;
+  int b, rows, page_count, columns, log2_page, prefix, slices;
+};
+
+// What one request takes: sane values whatever the arrays hold.
+struct Take {
+  int length, tokens;  // length -1: left out
+  int first, last;     // table columns [first, last) get new pages
+};
+
+__device__ __forceinline__ Take take_of(const TableArgs& a, int r) {
+  Take t{-1, 0, 0, 0};
+  if (r >= a.b) return t;
+  const int length = a.lengths[r], n = a.tokens ? a.tokens[r] : 1;
+  if (length < 0) return t;
+  t.length = length;
+  t.tokens = min(max(n, 0), a.rows);
+  const int mask = (1 << a.log2_page) - 1;
+  t.first = int(min((int64_t(length) + mask) >> a.log2_page, int64_t(a.columns)));
+  t.last = int(min((int64_t(length) + t.tokens + mask) >> a.log2_page, int64_t(a.columns)));
+  return t;
+}
+
+// Sum over the workgroup of x and y, in every thread.
+__device__ __forceinline__ void block_sum(int64_t& x, int64_t& y, int64_t (*s)[2]) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    x += __shfl_xor(x, o);
+    y += __shfl_xor(y, o);
+  }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) { s[wave][0] = x; s[wave][1] = y; }
+  __syncthreads();
+  x = y = 0;
+#pragma unroll
+  for (int w = 0; w < kTableThreads / 64; ++w) { x += s[w][0]; y += s[w][1]; }
+}
+
+// The largest i with s[i] <= x, for ascending s[0 .. kChunk] with s[0] <= x < s[kChunk].
+__device__ __forceinline__ int owner_of(const int64_t* s, int64_t x) {
+  int i = 0;
+#pragma unroll
+  for (int step = kChunk / 2; step > 0; step >>= 1)
+    if (s[i + step] <= x) i += step;
+  return i;
+}
+
+__global__ __launch_bounds__(kTableThreads) void batch_tables_kernel(TableArgs a) {
+  static_assert(kChunk == kTableThreads, "a thread per request of the chunk");
+  __shared__ int64_t s_tokens[kChunk + 1], s_pages[kChunk + 1];  // sums before each request of the chunk
+  __shared__ int s_length[kChunk], s_first[kChunk], s_last[kChunk];
+  __shared__ int64_t s_sum[kTableThreads / 64][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int chunk = int(blockIdx.x) / a.slices, slice = int(blockIdx.x) - chunk * a.slices;
+  const int r0 = chunk * kChunk;
+  const Take mine = take_of(a, r0 + tid);
+
+  int64_t tokens0 = 0, pages0 = 0;
+  if (chunk) {
+    for (int r = tid; r < r0; r += kTableThreads) {
+      const Take t = take_of(a, r);
+      tokens0 += t.tokens;
+      pages0 += t.last - t.first;
+    }
+    block_sum(tokens0, pages0, s_sum);
+    __syncthreads();
+  }
+
+  // inclusive sums within the wave, then the waves before
+  int64_t tokens = mine.tokens, pages = mine.last - mine.first;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t x = __shfl_up(tokens, o), y = __shfl_up(pages, o);
+    if (lane >= o) { tokens += x; pages += y; }
+  }
+  if (lane == 63) { s_sum[wave][0] = tokens; s_sum[wave][1] = pages; }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) { tokens += s_sum[w][0]; pages += s_sum[w][1]; }
+  tokens += tokens0;
+  pages += pages0;
+  s_tokens[tid + 1] = tokens;
+  s_pages[tid + 1] = pages;
+  if (tid == 0) { s_tokens[0] = tokens0; s_pages[0] = pages0; }
+  s_length[tid] = mine.length;
+  s_first[tid] = mine.first;
+  s_last[tid] = mine.last;
+  if (slice == 0) {
+    if (r0 + tid < a.b) a.cu_tokens[r0 + tid + 1] = int(min(tokens, int64_t(a.rows)));
+    if (chunk == 0 && tid == 0) a.cu_tokens[0] = 0;
+  }
+  __syncthreads();
+
+  const int mask = (1 << a.log2_page) - 1;
+  const int stride = a.slices * kTableThreads, begin = slice * kTableThreads + tid;
+  auto page_at = [&](int64_t j) { return j < a.page_count ? a.pages[j] : -1; };
+
+  // slots and positions of the chunk's tokens
+  const int64_t end = min(s_tokens[kChunk], int64_t(a.rows));
+  for (int64_t t = tokens0 + begin; t < end; t += stride) {
+    const int i = owner_of(s_tokens, t);
+    const int64_t p = s_length[i] + (t - s_tokens[i]);
+    const int64_t column = p >> a.log2_page;
+    int page = -1;
+    if (column < s_last[i])
+      page = column < s_first[i] ? a.table[int64_t(r0 + i) * a.columns + column] : page_at(s_pages[i] + column - s_first[i]);
+    a.slots[t] = page < 0 ? -1 : (int64_t(page) << a.log2_page) + (p & mask);
+    a.positions[t] = float(a.prefix + p);
+  }
+
+  // the chunk's new pages
+  for (int64_t j = pages0 + begin; j < s_pages[kChunk]; j += stride) {
+    const int i = owner_of(s_pages, j);
+    a.table[int64_t(r0 + i) * a.columns + s_first[i] + (j - s_pages[i])] = page_at(j);
+  }
+
+  // behind the pages of the requests that start with this step: -1
+  uint64_t starts = __ballot(mine.length == 0);
+  for (int turn = 0; starts; starts &= starts - 1, ++turn) {
+    if (turn % a.slices != slice) continue;
+    const int i = wave * 64 + __builtin_ctzll(starts);
+    for (int c = s_last[i] + lane; c < a.columns; c += 64) a.table[int64_t(r0 + i) * a.columns + c] = -1;
+  }
+
+  // rows behind the last request's tokens: no slot
+  if (r0 + kChunk >= a.b)
+    for (int64_t t = end + begin; t < a.rows; t += stride) a.slots[t] = -1;
+}
+
 bool valid_geometry(int max_pages, int max_slabs, int max_slots, int max_cols, int pps) {
   return max_pages > 0 && max_slabs > 0 && max_slots > 0 && max_cols > 0 && pps > 0 &&
          int64_t(max_slabs) * pps == max_pages && int64_t(max_slots) * max_cols <= INT32_MAX;
@@ -756,6 +905,27 @@ int mt_sched_decode_abort(MT_POOL_ARGS, const int* slots, int b, const int* new_
   MT_POOL_CHECK
   if (!slots || b < 1 || !new_page) return hipErrorInvalidValue;
   decode_abort_kernel<<<1, kThreads>>>(MT_POOL, slots, b, new_page);
+  return hipGetLastError();
+}
+
+int mt_sched_batch_tables(int* table, int64_t* slots, float* positions, int* cu_tokens, const int* lengths,
+                          const int* tokens, const int* pages, int b, int rows, int page_count, int columns,
+                          int page_size, int prefix_tokens) {
+  if (!table || !slots || !positions || !cu_tokens || !lengths || b < 1 || b > 65535 || rows < 1 || page_count < 0 ||
+      (page_count > 0 && !pages) || columns < 1 || int64_t(b) * columns > INT32_MAX ||
+      !(page_size == 8 || page_size == 16 || page_size == 32) || int64_t(columns) * page_size > INT32_MAX ||
+      prefix_tokens < 0)
+    return hipErrorInvalidValue;
+  TableArgs a{};
+  a.table = table; a.slots = slots; a.positions = positions; a.cu_tokens = cu_tokens;
+  a.lengths = lengths; a.tokens = tokens; a.pages = pages;
+  a.b = b; a.rows = rows; a.page_count = page_count; a.columns = columns; a.prefix = prefix_tokens;
+  a.log2_page = page_size == 8 ? 3 : page_size == 16 ? 4 : 5;
+  // Shares of a chunk: four tokens a thread, and about as much of the table where every request starts.
+  const int chunks = (b + kChunk - 1) / kChunk;
+  const int64_t work = int64_t(rows) + page_count;
+  a.slices = int(std::min<int64_t>(std::max<int64_t>(1, work / (int64_t(chunks) * kTableThreads * 4)), 1024));
+  batch_tables_kernel<<<chunks * a.slices, kTableThreads>>>(a);
   return hipGetLastError();
 }
 
