@@ -21,6 +21,7 @@ ARCH = 'gfx950'
 # time through an $ORIGIN rpath; that library is therefore built first.
 LIBRARIES = {
     'paged_attention_kernel': [],
+    'shared_prefix_kernel': [],
     'inference_kernels': [],
     'cuda_runtime': [],
     'sched_kernels': [],

@@ -3,8 +3,8 @@
 Argument order and meaning follow the reference's ctypes call sites
 (minitorch/paged_kv_cache.py:205-221, minitorch/paged_decode.py:65-69,
 minitorch/kv_cache.py:35,52, minitorch/pretrained_gpt2.py:30-31). Every call
-goes to ``cuda_kernels/paged_attention_kernel.so`` or
-``cuda_kernels/inference_kernels.so``.
+goes to ``cuda_kernels/paged_attention_kernel.so``, ``shared_prefix_kernel.so``
+(a batch behind a shared prefix), ``sched_kernels.so`` or ``inference_kernels.so``.
 """
 import ctypes as ct
 from functools import lru_cache
@@ -15,6 +15,10 @@ from .dtypes import dtype_code
 
 def paged_library():
     return library('paged_attention_kernel')
+
+
+def shared_library():
+    return library('shared_prefix_kernel')
 
 
 def inference_library():
@@ -164,6 +168,57 @@ def _small_work_list(lengths, heads, compute_units):
     work[0::2] = order
     work[1::2] = 0
     return work, len(order), 0
+
+
+def batch_tables(table, slots, positions, cu_tokens, lengths, tokens, pages, *, b, rows, page_count, columns,
+                 page_size, prefix_tokens=0):
+    """``mt_sched_batch_tables``: the block tables (in and out), slot map,
+    positions and token offsets of a step whose request ``r`` holds
+    ``lengths[r]`` tokens and gets ``tokens[r]`` more (``tokens`` None: one
+    each), their pages taken in request order from the flat list ``pages``;
+    ``rows`` entries of ``slots`` (int64) and ``positions`` (fp32)."""
+    call(library('sched_kernels'), 'mt_sched_batch_tables', [P] * 7 + [I] * 6, table, slots, positions, cu_tokens,
+         lengths, tokens, pages, b, rows, page_count, columns, page_size, prefix_tokens)
+
+
+def paged_append_slots(k, v, slab_table, slots, *, rows, h, d, page_size, pages_per_slab, num_slabs, layer, layers,
+                       dtype, kv_stride=0):
+    """``mt_paged_append_slots``: K/V rows [rows, kv_stride] to their pages
+    through the slot map of :func:`batch_tables`."""
+    call(shared_library(), 'mt_paged_append_slots', [P] * 4 + [I] * 10, k, v, slab_table, slots, rows, h, d, page_size,
+         pages_per_slab, num_slabs, layer, layers, dtype_code(dtype), kv_stride)
+
+
+@lru_cache(maxsize=4096)
+def shared_workspace_bytes(*, rows, b, h, d, page_size, prefix_tokens, columns, max_tokens, dtype):
+    """Workspace size for :func:`paged_shared_decode` (rows = b, max_tokens 1)
+    and :func:`paged_shared_attention` (0 when none is needed); a pure function
+    of its arguments on one device, memoized."""
+    out = ct.c_size_t()
+    call(shared_library(), 'mt_paged_shared_workspace_bytes', [I] * 9 + [ct.POINTER(ct.c_size_t)], rows, b, h, d,
+         page_size, prefix_tokens, columns, max_tokens, dtype_code(dtype), ct.byref(out))
+    return out.value
+
+
+def paged_shared_decode(out, q, k, v, slab_table, prefix_table, block_table, offsets, *, b, h, d, page_size,
+                        pages_per_slab, num_slabs, prefix_tokens, columns, layer, layers, dtype, qkv_stride=0,
+                        workspace=None, workspace_bytes=0):
+    """``mt_paged_shared_decode``: append and attention of one token per request
+    over a prefix that the batch shares and the request's own pages."""
+    call(shared_library(), 'mt_paged_shared_decode', [P] * 8 + [I] * 12 + [P, Z], out, q, k, v, slab_table,
+         prefix_table, block_table, offsets, b, h, d, page_size, pages_per_slab, num_slabs, prefix_tokens, columns,
+         layer, layers, dtype_code(dtype), qkv_stride, workspace, workspace_bytes)
+
+
+def paged_shared_attention(out, q, slab_table, prefix_table, block_table, lengths, cu_tokens, *, b, rows, max_tokens,
+                           h, d, page_size, pages_per_slab, num_slabs, prefix_tokens, columns, layer, layers, dtype,
+                           q_stride=0, out_stride=0, workspace=None, workspace_bytes=0):
+    """``mt_paged_shared_attention``: attention of several new tokens per
+    request, appended already, over a shared prefix and, causally, the request's
+    own pages; token-major rows q [rows, q_stride] and out [rows, out_stride]."""
+    call(shared_library(), 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], out, q, slab_table, prefix_table,
+         block_table, lengths, cu_tokens, b, rows, max_tokens, h, d, page_size, pages_per_slab, num_slabs,
+         prefix_tokens, columns, layer, layers, dtype_code(dtype), q_stride, out_stride, workspace, workspace_bytes)
 
 
 def embedding_gather(dst, weights, ids, tokens, vocab, dim):
