@@ -195,18 +195,852 @@ __global__ __launch_bounds__(256) void shared_walk_kernel(SharedArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// The fast path. A launch holds two kinds of work, whose results are partial:
+// (accumulators, maximum, denominator) per query, head and piece of the keys,
+// joined by merge_kernel.
+//   * A prefix item attends a tile of 32 QT queries of one head -- of whatever
+//     requests -- to a piece of the prefix, on the matrix cores: the piece is
+//     read once for all of them.
+//   * An own item attends a request's queries to its own pages: one query on the
+//     VALU, streaming (decode), several on the matrix cores, causally.
+// The first is bound by the matrix cores and the VALU between them, the second by
+// memory, so that one launch that mixes them runs both at once.
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kPages = 512;  // pages of an item's keys, resolved into LDS
+constexpr float kRescale = 6.f;
+constexpr float kHalfShift = 9.f;  // 2^(kRescale + kHalfShift) is below fp16's largest
+
+// How the launch is cut (made on the host).
+struct Plan {
+  // prefix: tiles of 32 qt queries, pieces of piece_keys keys (a multiple of 32)
+  int qt, tiles, pieces, piece_keys;
+  int64_t prefix_items;
+  // own keys: splits of split_keys
+  int split_keys, splits;
+  // decode: waves per item and workgroups that take the splits past a row's first
+  int item_waves, more_blocks;
+  // several queries: tiles of 32 own_qt queries
+  int own_qt, own_tiles;
+  int64_t own_blocks;
+  float* partials;
+};
+
+// Elements of a query's partial: accumulators, maximum and denominator, 16-byte aligned.
+template <int DP>
+constexpr int part_row() { return DP + 4; }
+
+template <int DP>
+__device__ __forceinline__ float* part_of(const SharedArgs& a, const Plan& p, int piece, int head, int64_t row) {
+  return p.partials + ((int64_t(piece) * a.g.heads + head) * a.rows + row) * part_row<DP>();
+}
+
+// Staged keys of a workgroup of eight waves: two halves of kHalf keys, K and V
+// each. A wave takes blocks of 32 keys: with few waves per query group (KG <=
+// kHalf / 32) a round is one half, staged while the other is computed; with more,
+// both halves at once.
+template <int DT, int DP>
+struct Shape {
+  static constexpr int ES = elem_bytes<DT>();
+  static constexpr int EC = 16 / ES;          // elements per 16-byte chunk
+  static constexpr int CPR = DP / EC;         // chunks per row
+  static constexpr int RW = kWave / CPR;      // rows one load instruction of a wave fills
+  static constexpr int kRowBytes = DP * ES;
+  static constexpr int kHalf = kRowBytes == 512 ? 64 : 128;
+  static constexpr int kBlocks = kHalf / 32;
+  static constexpr int kPlane = kHalf * kRowBytes;
+  static constexpr int NC = kHalf / (kWaves * RW);  // loads per lane, K and V each
+  static constexpr int DT32 = DP / 32;
+  static constexpr int QW = DT == kF32 ? DP / 8 : DP / 16;  // 16-byte query registers
+  static constexpr int OS = DP + 4;
+  static constexpr size_t kMerge = size_t(kWaves) * 32 * (OS + 2) * sizeof(float);
+  static constexpr size_t kLds = size_t(4) * kPlane > kMerge ? size_t(4) * kPlane : kMerge;
+  static constexpr int SW = kRowBytes == 128 ? 4 : 2;  // waves per SIMD: two workgroups a compute unit, or one
+  // Chunk p of key row r lies at chunk kpos / vpos of the row (both their own
+  // inverse), so that the reads below are free of bank conflicts: K 16 bytes of
+  // 32 consecutive rows, V 4 rows x 64 bytes (16-bit) or two rows 4 apart x 128
+  // bytes (fp32).
+  static __device__ __forceinline__ int kpos(int r, int p) { return CPR == 8 ? p ^ ((r >> 1) & 7) : p ^ (r & 15); }
+  static __device__ __forceinline__ int vpos(int r, int p) {
+    if constexpr (DT == kF32) return p ^ (((r >> 2) & 1) << 3);
+    else return CPR == 8 ? p ^ (((r >> 1) & 1) << 2) : p ^ ((r & 3) << 2);
+  }
+};
+
+// A tile of queries and the keys [k0, k1) of a table row that it attends (k0 a
+// multiple of 32, at most kPages pages): query j those up to limit + j.
+struct Tile {
+  const void* q;  // row of query 0, at the head's columns
+  int nq, qt;
+  const int* table_row;
+  int columns, k0, k1;
+  int64_t limit;
+  float* part;  // partial of query 0 (the others follow)
+};
+
+// S^T = K Q^T in 32x32 MFMAs (keys x queries: two lanes share a query and hold
+// half of a block's scores of it each), online softmax in registers, O^T += V^T
+// P^T with the scores' own layout as the B operand. For 16-bit types P is split
+// into a high and a low part of the type (two MFMAs), so that the weights keep 16
+// (bf16) or 22 (fp16) bits and the output is as exact as the other attention
+// kernels'; fp16's are taken 2^kHalfShift larger, whose low parts would
+// otherwise end at 2^-24. The exponentials' reference moves when a score exceeds
+// it by kRescale only.
+template <int DT, int DP>
+__device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, int head, char* s_raw,
+                                            typename Elem<DT>::T const** s_page, int* s_missing) {
+  using T = typename Elem<DT>::T;
+  using S = Shape<DT, DP>;
+  constexpr int EC = S::EC, CPR = S::CPR, NC = S::NC, DT32 = S::DT32, QW = S::QW;
+  constexpr float kShift = DT == kF16 ? kHalfShift : 0.f;
+  constexpr int CH = DP == 64 ? 4 : 2;  // chains of an fp32 block's sums
+  const Geometry& g = a.g;
+  const int dim = g.dim, chunks = dim / EC;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qt_n = t.qt, kg_n = kWaves / qt_n;
+  const int kg = wave / qt_n, qt = wave - kg * qt_n;
+  const int grp = lane >> 5, col = lane & 31;
+  const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)s_raw));
+
+  // B operand of S^T: 16-bit types dims [16 s + 8 grp, + 8) of the lane's query,
+  // fp32 dims [DP / 2 * grp, + DP / 2).
+  const int q0 = qt * 32, qi = q0 + col;
+  const bool live = q0 < t.nq;
+  const T* qrow = static_cast<const T*>(t.q) + (qi < t.nq ? qi : 0) * a.q_r;
+  u32x4 qv[QW];
+#pragma unroll
+  for (int s = 0; s < QW; ++s) {
+    const int p = DT == kF32 ? CPR / 2 * grp + s : 2 * s + grp;
+    qv[s] = *global_view(reinterpret_cast<const u32x4*>(p < chunks ? qrow + p * EC : reinterpret_cast<const T*>(g_fill + 4)));
+  }
+
+  // the pages of the keys
+  const int pages = (t.k1 - t.k0 + g.page_size - 1) >> g.log2_page;
+  if (tid == 0) *s_missing = 0;
+  __syncthreads();
+  for (int j = tid; j < pages; j += kThreads) {
+    const int column = (t.k0 >> g.log2_page) + j;
+    const T* page = column < t.columns ? resolve_page<T>(a.slabs, t.table_row[column], g, head) : nullptr;
+    s_page[j] = page;
+    if (!page) *s_missing = 1;
+  }
+  __syncthreads();
+  const bool plain = !*s_missing && chunks == CPR;
+
+  // Keys [k, k + kHalf) into half `h`. Keys past the end are zero; a missing
+  // page is NaN in K (its scores are NaN) and zero in V.
+  const int sr = wave * S::RW + lane / CPR, spos = lane % CPR;
+  auto stage = [&](int k, int h) {
+    const uint32_t lk = lds0 + h * 2 * S::kPlane + wave * 1024, lv = lk + S::kPlane;
+    if (plain && k + S::kHalf <= t.k1) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int r = sr + n * kWaves * S::RW;
+        const T* page = s_page[(k + r - t.k0) >> g.log2_page] + (r & (g.page_size - 1)) * dim;
+        stage16(page + S::kpos(r, spos) * EC, lk + n * kWaves * 1024);
+        stage16(page + g.kind_stride + S::vpos(r, spos) * EC, lv + n * kWaves * 1024);
+      }
+    } else {
+      int row = sr;
+      asm volatile("" : "+v"(row));  // keeps this rarer path's terms out of the registers of the loop
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int r = row + n * kWaves * S::RW, key = k + r;
+        // a block wholly past the keys is never read
+        if (k + ((wave * S::RW + n * kWaves * S::RW) & ~31) >= t.k1) continue;
+        const int pk = S::kpos(r, spos), pv = S::vpos(r, spos);
+        const T* kp = reinterpret_cast<const T*>(g_fill + 4);
+        const T* vp = kp;
+        if (key < t.k1) {
+          const T* page = s_page[(key - t.k0) >> g.log2_page];
+          if (!page) {
+            kp = reinterpret_cast<const T*>(g_fill);
+          } else {
+            page += (r & (g.page_size - 1)) * dim;
+            if (pk < chunks) kp = page + pk * EC;
+            if (pv < chunks) vp = page + g.kind_stride + pv * EC;
+          }
+        }
+        stage16(kp, lk + n * kWaves * 1024);
+        stage16(vp, lv + n * kWaves * 1024);
+      }
+    }
+  };
+
+  float m = -INFINITY, l = 0.f;
+  floatx16 o[DT32];
+#pragma unroll
+  for (int d = 0; d < DT32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  const int64_t own_limit = t.limit + qi;
+  const int last_key = int(own_limit < t.k1 ? own_limit : t.k1 - 1);  // of this lane's query
+
+  // One block of 32 keys from `base` on, at row `at` of half h.
+  auto block = [&](int base, int h, int at) {
+    const T* const s_k = reinterpret_cast<const T*>(s_raw + h * 2 * S::kPlane) + at * DP;
+    const T* const s_v = s_k + S::kPlane / S::ES;
+    // lane holds keys base + 8 (i / 4) + 4 grp + i % 4 of query qi
+    floatx16 sc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+    auto read_k = [&](int s) {
+      const int p = DT == kF32 ? CPR / 2 * grp + s : 2 * s + grp;
+      return *reinterpret_cast<const u32x4*>(s_k + col * DP + S::kpos(col, p) * EC);
+    };
+    if constexpr (DT == kF32) {
+      // short chains of sums
+      floatx16 part[CH];
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[j][i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < QW; ++s) {
+        const u32x4 kf = read_k(s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          floatx16& c = part[j % CH];
+          c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[j]), __uint_as_float(qv[s][j]), c, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = CH == 4 ? (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]) : part[0][i] + part[1][i];
+    } else {
+#pragma unroll
+      for (int s = 0; s < QW; ++s) sc = mfma32<DT>(read_k(s), qv[s], sc);
+    }
+    // limits, only for blocks that reach past one (a wave-uniform test)
+    if (base + 31 > t.limit + q0 || base + 32 > t.k1) {
+      const int last = last_key - base - 4 * grp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) > last) sc[i] = -INFINITY;
+    }
+    float top = sc[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);  // NaN scores are dropped
+    top = max_halves(top) * a.qscale;
+    if (__any(top > m + kRescale)) {  // also a query's first keys, m = -inf
+      const float mn = fmaxf(m, top);
+      const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+      m = mn;
+    }
+    const float ref = m == -INFINITY ? 0.f : m - kShift;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = fast_exp2(fmaf(sc[i], a.qscale, -ref));
+    float sum[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = sc[i] + sc[i + 8];
+#pragma unroll
+    for (int w = 4; w > 0; w /= 2)
+#pragma unroll
+      for (int i = 0; i < w; ++i) sum[i] += sum[i + w];
+    l += sum[0];
+    if constexpr (DT == kF32) {
+      // a block's sums start at zero, in chains, and are added to the running ones
+#pragma unroll
+      for (int d = 0; d < DT32; ++d) {
+        floatx16 ob[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ob[j][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int rr = 8 * (i >> 2) + 4 * grp + (i & 3), dd = 32 * d + col;
+          const float vv = s_v[rr * DP + S::vpos(rr, dd >> 2) * 4 + (dd & 3)];
+          ob[i % CH] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv, sc[i], ob[i % CH], 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          o[d][i] += CH == 4 ? (ob[0][i] + ob[1][i]) + (ob[2][i] + ob[3][i]) : ob[0][i] + ob[1][i];
+      }
+    } else {
+      // 16 keys a step: slot j < 4 of a lane holds key 16 s + 4 grp + j, slot j
+      // >= 4 key 16 s + 8 + 4 grp + j - 4, in P as in V^T
+      const int t16 = lane & 15;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t h2, l2;
+          SplitP<DT>::split(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
+          hi[w] = h2;
+          lo[w] = l2;
+        }
+#pragma unroll
+        for (int d = 0; d < DT32; ++d) {
+          const int rr = 4 * grp + (t16 >> 2);
+          const int p = 4 * d + ((lane >> 4) & 1) * 2 + ((t16 & 3) >> 1);
+          const T* v_at = s_v + (16 * s + rr) * DP + S::vpos(rr, p) * 8 + (t16 & 1) * 4;
+          const uint2 x = read_transposed(v_at), y = read_transposed(v_at + 8 * DP);
+          const u32x4 vv = {x.x, x.y, y.x, y.y};
+          o[d] = mfma32<DT>(vv, hi, o[d]);
+          o[d] = mfma32<DT>(vv, lo, o[d]);
+        }
+      }
+    }
+  };
+
+  const bool both = kg_n > S::kBlocks;  // rounds of both halves
+  stage(t.k0, 0);
+  if (both && t.k0 + S::kHalf < t.k1) stage(t.k0 + S::kHalf, 1);
+#pragma unroll
+  for (int s = 0; s < QW; ++s) asm volatile("" : "+v"(qv[s]));  // the query has arrived before the loop
+  if (both) {
+    const int h = kg / S::kBlocks, at = (kg - h * S::kBlocks) * 32;
+    for (int k = t.k0; k < t.k1; k += 2 * S::kHalf) {
+      wait_staged<0>();
+      __syncthreads();
+      const int base = k + h * S::kHalf + at;
+      if (live && h < 2 && base < t.k1 && base <= t.limit + min(q0 + 31, t.nq - 1)) block(base, h, at);
+      const int next = k + 2 * S::kHalf;
+      if (next < t.k1) {
+        __syncthreads();
+        stage(next, 0);
+        if (next + S::kHalf < t.k1) stage(next + S::kHalf, 1);
+      }
+    }
+  } else {
+    int h = 0;
+    for (int k = t.k0; k < t.k1; k += S::kHalf, h ^= 1) {
+      wait_staged<0>();
+      __syncthreads();  // the half's keys are there, and the half before is done with
+      if (k + S::kHalf < t.k1) stage(k + S::kHalf, h ^ 1);
+      if (live)
+        for (int at = kg * 32; at < S::kHalf; at += kg_n * 32) {
+          const int base = k + at;
+          if (base >= t.k1 || base > t.limit + min(q0 + 31, t.nq - 1)) break;
+          block(base, h, at);
+        }
+    }
+  }
+
+  // The waves that share queries meet in LDS; then every thread joins four dims
+  // of a query. O^T lane layout: dims 32 d + 8 (i / 4) + 4 grp + i % 4 of query qi.
+  l = add_halves(l);
+  m -= kShift;
+  constexpr int R = part_row<DP>();
+  if (kg_n == 1) {
+    if (qi < t.nq) {
+      float* row = t.part + qi * R;
+#pragma unroll
+      for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(row + 32 * d + 2 * i + 4 * grp) = float4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+      if (grp == 0) *reinterpret_cast<float2*>(row + DP) = float2{m, l};
+    }
+    return;
+  }
+  float* const s_o = reinterpret_cast<float*>(s_raw);
+  float2* const s_ml = reinterpret_cast<float2*>(s_o + kWaves * 32 * S::OS);
+  const int tq = 32 * qt_n;
+  __syncthreads();
+  {
+    float* row = s_o + (kg * tq + qi) * S::OS + 4 * grp;
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(row + 32 * d + 2 * i) = float4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+    if (grp == 0) s_ml[kg * tq + qi] = float2{m, l};
+  }
+  __syncthreads();
+  for (int u = tid; u < t.nq * (DP / 4); u += kThreads) {
+    const int q = u / (DP / 4), dd = 4 * (u - q * (DP / 4));
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < kg_n; ++k) M = fmaxf(M, s_ml[k * tq + q].x);
+    float4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < kg_n; ++k) {
+      const float2 ml = s_ml[k * tq + q];
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+      const float4 x = *reinterpret_cast<const float4*>(s_o + (k * tq + q) * S::OS + dd);
+      L = fmaf(ml.y, w, L);  // a NaN denominator (missing page) stays
+      if (isnan(ml.y)) L = NAN;
+      acc.x = fmaf(x.x, w, acc.x); acc.y = fmaf(x.y, w, acc.y);
+      acc.z = fmaf(x.z, w, acc.z); acc.w = fmaf(x.w, w, acc.w);
+    }
+    *reinterpret_cast<float4*>(t.part + q * R + dd) = acc;
+    if (dd == 0) *reinterpret_cast<float2*>(t.part + q * R + DP) = float2{M, L};
+  }
+}
+
+// Own keys of one query (decode), streamed: a wave covers 8 tokens a step, eight
+// lanes a token, U steps in flight; item_waves waves share an item. The keys of
+// split `split` of row `row`; the last split appends and scores the new token.
+// All threads of the workgroup enter (barriers); `on` where the group has an item.
+template <int DT, int DP, Rows FULL>
+__device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, bool on, int row, int head, int split,
+                                            float* s_state) {
+  using T = typename Elem<DT>::T;
+  constexpr int G = 8, DL = DP / G, RB = kWave / G;
+  constexpr int U = DL * elem_bytes<DT>() >= 64 ? 1 : DL * elem_bytes<DT>() >= 32 ? 2 : 4;
+  using C = Chunk<DT, DL, FULL, G>;
+  const Geometry& g = a.g;
+  const int dim = FULL == kRowsFull ? DP : g.dim;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & (kWave - 1);
+  const int W = p.item_waves, gw = wave % W, first_wave = wave - gw;
+  const int col0 = C::first_col(lane % G), tok = lane / G;
+  Softmax<DL, G> st;
+  st.init();
+  int nsplit = 1;
+  if (on) {
+    const int offset = a.lengths[row];
+    const int64_t L = int64_t(offset) + 1, cap = int64_t(g.columns) * g.page_size;
+    on = offset >= 0 && L <= cap;
+    if (on) nsplit = int((uint32_t(L) + uint32_t(p.split_keys) - 1) / uint32_t(p.split_keys));
+    on = on && split < nsplit;
+    if (on) {
+      const int t0 = split * p.split_keys, t1 = int(L < int64_t(t0) + p.split_keys ? L : int64_t(t0) + p.split_keys);
+      const bool owns_new = split == nsplit - 1;
+      const int ntok = (owns_new ? t1 - 1 : t1) - t0;
+      const int* table_row = a.table + int64_t(row) * g.columns;
+      const int64_t qrow = int64_t(row) * a.q_r + int64_t(head) * dim;
+      Query<DT, DP, FULL, G> qv;
+      qv.load(static_cast<const T*>(a.q) + qrow, col0, dim, a.qscale);
+      // lane i: the page of this wave's step i
+      const int rel0 = (gw + W * lane) * RB;
+      const T* page = nullptr;
+      if (rel0 < ntok) page = resolve_page<T>(a.slabs, table_row[(t0 + rel0) >> g.log2_page], g, head);
+      const uint64_t at = reinterpret_cast<uintptr_t>(page);
+      const int at_lo = int(uint32_t(at)), at_hi = int(uint32_t(at >> 32));
+      const int steps_all = (ntok + RB - 1) / RB;
+      const int steps = steps_all > gw ? (steps_all - gw + W - 1) / W : 0;
+      for (int i0 = 0; i0 < steps; i0 += U) {
+        C kc[U], vc[U];
+        bool valid[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = min(i0 + u, kWave - 1);
+          const int rel = (gw + W * (i0 + u)) * RB + tok;
+          valid[u] = rel < ntok;
+          const T* base = reinterpret_cast<const T*>(uint64_t(uint32_t(__builtin_amdgcn_readlane(at_hi, i))) << 32 |
+                                                     uint32_t(__builtin_amdgcn_readlane(at_lo, i)));
+          if (valid[u] && base) {
+            const T* kp = base + ((t0 + rel) & (g.page_size - 1)) * dim + col0;
+            kc[u].template load<true>(kp, col0, dim);
+            vc[u].template load<true>(kp + g.kind_stride, col0, dim);
+          } else {
+            kc[u].nan_fill();
+            vc[u].nan_fill();
+          }
+        }
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = qv.score(kc[u]);
+        // one move of the running maximum for the U tokens; no scores but -Inf leave it
+        float top = st.m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (valid[u]) top = fmaxf(top, s[u]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float alpha = fast_exp2(st.m - ref);
+        st.l *= alpha;
+#pragma unroll
+        for (int e = 0; e < DL; ++e) st.acc[e] *= alpha;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (!valid[u]) continue;
+          const float w = fast_exp2(s[u] - ref);
+          float vf[DL];
+          vc[u].to_float(vf);
+          st.l += w;
+#pragma unroll
+          for (int e = 0; e < DL; ++e) st.acc[e] = fmaf(w, vf[e], st.acc[e]);
+        }
+        st.m = top;
+      }
+      if (owns_new && gw == 0) {
+        // the new token, by the first eight lanes: written to its page and scored
+        const int last = t1 - 1;
+        const T* np = resolve_page<T>(a.slabs, table_row[last >> g.log2_page], g, head);
+        C kn, vn;
+        kn.load(static_cast<const T*>(a.k) + qrow + col0, col0, dim);
+        vn.load(static_cast<const T*>(a.v) + qrow + col0, col0, dim);
+        if (np && lane < G) {
+          T* kp = const_cast<T*>(np) + (last & (g.page_size - 1)) * dim + col0;
+          T* vp = kp + g.kind_stride;
+#pragma unroll
+          for (int i = 0; i < C::NV; ++i) {
+            if (FULL == kRowsPadded && col0 + i * G * per16<DT>() >= dim) break;
+            global_view(reinterpret_cast<u32x4*>(kp))[i * G] = kn.raw[i];
+            global_view(reinterpret_cast<u32x4*>(vp))[i * G] = vn.raw[i];
+          }
+        }
+        if (!np) { kn.nan_fill(); vn.nan_fill(); }
+        const float sc = qv.score(kn);
+        if (lane < G) {
+          float vf[DL];
+          vn.to_float(vf);
+          const float top = fmaxf(st.m, sc), ref = top == -INFINITY ? 0.f : top;
+          const float alpha = fast_exp2(st.m - ref), w = fast_exp2(sc - ref);
+          st.l = fmaf(st.l, alpha, w);
+#pragma unroll
+          for (int e = 0; e < DL; ++e) st.acc[e] = fmaf(w, vf[e], st.acc[e] * alpha);
+          st.m = top;
+        }
+      }
+    }
+  }
+  // States of the 16-lane rows by DPP, then the item's 4 W of them in LDS.
+  float* const s_acc = s_state;                            // [32][DP]
+  float2* const s_ml = reinterpret_cast<float2*>(s_state + 4 * kWaves * DP);
+  st.row_merge();
+  if ((lane & 15) < G) {
+    const int si = wave * 4 + (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < DL; ++i) s_acc[si * DP + col0 + C::col_of(i)] = st.acc[i];
+    if ((lane & 15) == 0) s_ml[si] = float2{st.m, st.l};
+  }
+  __syncthreads();
+  if (on) {
+    float* part = part_of<DP>(a, p, p.pieces + split, head, row);
+    for (int d = gw * kWave + lane; d < DP; d += W * kWave) {
+      float M = -INFINITY, L = 0.f, acc = 0.f;
+      for (int j = first_wave * 4; j < (first_wave + W) * 4; ++j) M = fmaxf(M, s_ml[j].x);
+      for (int j = first_wave * 4; j < (first_wave + W) * 4; ++j) {
+        const float2 ml = s_ml[j];
+        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+        L = fmaf(ml.y, w, L);
+        if (isnan(ml.y)) L = NAN;  // also where no score was a number
+        acc = fmaf(s_acc[j * DP + d], w, acc);
+      }
+      part[d] = acc;
+      if (d == 0) { part[DP] = M; part[DP + 1] = L; }
+    }
+  }
+  __syncthreads();
+}
+
+// Splits past the first of a decode's long rows: every workgroup counts them (rows
+// in chunks of a thread each) and takes its share, eight waves at a time.
+template <int DT, int DP, Rows FULL>
+__device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, int block, float* s_state, int* s_count) {
+  const Geometry& g = a.g;
+  const int tid = threadIdx.x, groups = kWaves / p.item_waves, group = (tid >> 6) / p.item_waves;
+  const int64_t cap = int64_t(g.columns) * g.page_size;
+  int64_t set = block;  // this workgroup's next set of `groups` items, less those of the chunks before
+  for (int r0 = 0; r0 < a.b; r0 += kThreads) {
+    int more = 0;
+    if (r0 + tid < a.b) {
+      const int64_t L = int64_t(a.lengths[r0 + tid]) + 1;
+      if (L > p.split_keys && L <= cap) more = int((L - 1) / p.split_keys);
+    }
+    // inclusive sums over the chunk
+    int sum = wave_inclusive_add(more);
+    __syncthreads();
+    if ((tid & 63) == 63) s_count[kThreads + (tid >> 6)] = sum;
+    __syncthreads();
+    for (int w = 0; w < (tid >> 6); ++w) sum += s_count[kThreads + w];
+    s_count[tid] = sum;
+    __syncthreads();
+    const int64_t items = int64_t(s_count[kThreads - 1]) * g.heads;
+    const int64_t sets = (items + groups - 1) / groups;
+    for (; set < sets; set += p.more_blocks) {
+      const int64_t item = set * groups + group;
+      const bool on = item < items;
+      const int x = on ? int(item / g.heads) : 0, head = on ? int(item - int64_t(x) * g.heads) : 0;
+      int i = 0;  // the first row whose sum passes x
+#pragma unroll
+      for (int step = kThreads / 2; step > 0; step >>= 1)
+        if (s_count[i + step - 1] <= x) i += step;
+      const int before = i ? s_count[i - 1] : 0;
+      stream_item<DT, DP, FULL>(a, p, on, r0 + i, head, 1 + x - before, s_state);
+    }
+    set -= sets;
+  }
+}
+
+// Which item a workgroup works on: `count` of `all` workgroups are of the first
+// kind, spread evenly. Returns the index among its kind.
+__device__ __forceinline__ bool spread(int64_t block, int64_t count, int64_t all, int& index) {
+  const int64_t before = block * count / all, upto = (block + 1) * count / all;
+  index = int(upto > before ? before : block - before);
+  return upto > before;
+}
+
+template <int DT, int DP, Rows FULL, bool DECODE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(Shape<DT, DP>::SW)))
+void shared_kernel(SharedArgs a, Plan p) {
+  using T = typename Elem<DT>::T;
+  using S = Shape<DT, DP>;
+  __shared__ const T* s_page[kPages];
+  __shared__ int s_missing;
+  __shared__ __align__(16) char s_raw[S::kLds];
+  const Geometry& g = a.g;
+  int block = int(blockIdx.x);
+  if constexpr (DECODE) {
+    if (block < p.more_blocks) {
+      stream_more<DT, DP, FULL>(a, p, block, reinterpret_cast<float*>(s_raw), reinterpret_cast<int*>(s_page));
+      return;
+    }
+    block -= p.more_blocks;
+  }
+  int index;
+  if (spread(block, p.prefix_items, p.prefix_items + p.own_blocks, index)) {
+    // (piece, head, tile), the tiles of a piece side by side
+    const int ph = index / p.tiles, tile = index - ph * p.tiles;
+    const int piece = ph / g.heads, head = ph - piece * g.heads;
+    const int64_t row = int64_t(tile) * 32 * p.qt;
+    Tile t;
+    t.q = static_cast<const T*>(a.q) + row * a.q_r + int64_t(head) * g.dim;
+    t.nq = int(min(int64_t(32 * p.qt), a.rows - row));
+    t.qt = p.qt;
+    t.table_row = a.prefix_table;
+    t.columns = a.prefix_columns;
+    t.k0 = piece * p.piece_keys;
+    t.k1 = min(a.prefix, t.k0 + p.piece_keys);
+    t.limit = INT_MAX;
+    t.part = part_of<DP>(a, p, piece, head, row);
+    attend_tile<DT, DP>(a, t, head, s_raw, s_page, &s_missing);
+    return;
+  }
+  if constexpr (DECODE) {
+    const int groups = kWaves / p.item_waves;
+    const int64_t item = int64_t(index) * groups + (threadIdx.x >> 6) / p.item_waves;
+    const bool on = item < int64_t(a.b) * g.heads;
+    const int row = on ? int(item / g.heads) : 0;
+    stream_item<DT, DP, FULL>(a, p, on, row, int(item - int64_t(row) * g.heads), 0, reinterpret_cast<float*>(s_raw));
+  } else {
+    // (split, request, tile, head)
+    int i = index / g.heads;
+    const int head = index - i * g.heads;
+    const int rt = i / p.own_tiles, tile = i - rt * p.own_tiles;
+    const int split = rt / a.b, r = rt - split * a.b;
+    const Request rq = request_of(a, r);
+    const int q0 = tile * 32 * p.own_qt;
+    if (rq.length < 0 || q0 >= rq.tokens) return;
+    Tile t;
+    t.nq = min(32 * p.own_qt, rq.tokens - q0);
+    // a key past the table is a missing page: one of them is enough
+    const int64_t end = min(int64_t(rq.length) + q0 + t.nq, int64_t(g.columns) * g.page_size + 1);
+    const int64_t k0 = int64_t(split) * p.split_keys;
+    if (k0 >= end) return;
+    const int64_t row = int64_t(rq.row0) + q0;
+    t.q = static_cast<const T*>(a.q) + row * a.q_r + int64_t(head) * g.dim;
+    t.qt = p.own_qt;
+    t.table_row = a.table + int64_t(r) * g.columns;
+    t.columns = g.columns;
+    t.k0 = int(k0);
+    t.k1 = int(min(end, k0 + p.split_keys));
+    t.limit = int64_t(rq.length) + q0;
+    t.part = part_of<DP>(a, p, p.pieces + split, head, row);
+    attend_tile<DT, DP>(a, t, head, s_raw, s_page, &s_missing);
+  }
+}
+
+// Joins the pieces of every query: DP / 4 lanes a (row, head), four dims each. A
+// query left non-finite, and not by a missing page (whose NaN is the
+// denominator's too), is attended once more by a wave on the VALU: on the matrix
+// cores a key that a query does not attend has weight 0, and 0 * Inf or 0 * NaN of
+// its V is NaN, and so is the 0 * Inf of a weight's low part.
+constexpr int kMergeThreads = 256;
+template <int DT, int DP>
+__global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedArgs a, Plan p) {
+  using T = typename Elem<DT>::T;
+  constexpr int LANES = DP / 4, PER = kMergeThreads / LANES;  // (row, head) pairs a workgroup
+  __shared__ int s_count[kMergeThreads / kWave];
+  const Geometry& g = a.g;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int64_t pair0 = int64_t(blockIdx.x) * PER, pair = pair0 + tid / LANES;
+  const int64_t row = pair / g.heads;
+  const int head = int(pair - row * g.heads), dd = 4 * (tid % LANES);
+  int r = int(row);
+  if (a.cu_tokens) {
+    // the request of the workgroup's first row: as many as start at or before it,
+    // less one; of a later row by bisection from there
+    const int64_t row0 = pair0 / g.heads;
+    int n = 0;
+    for (int j = tid; j < a.b; j += kMergeThreads) n += a.cu_tokens[j] <= row0;
+#pragma unroll
+    for (int w = kWave / 2; w > 0; w /= 2) n += __shfl_xor(n, w);
+    if (lane == 0) s_count[tid >> 6] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < kMergeThreads / kWave; ++w) n += s_count[w];
+    r = max(n - 1, 0);
+    if (row < a.rows && r + 1 < a.b && a.cu_tokens[r + 1] <= row) {
+      int above = a.b;
+      while (r + 1 < above) {
+        const int mid = (r + above) / 2;
+        if (a.cu_tokens[mid] <= row) r = mid;
+        else above = mid;
+      }
+    }
+  }
+  // what the row attends; own keys in `splits` pieces
+  bool write = row < a.rows, padding = false;
+  int splits = 0, i = 0;
+  Request rq{0, 0, 0};
+  float L = 0.f;
+  if (write) {
+    rq = request_of(a, r);
+    i = int(row - rq.row0);
+    write = row >= rq.row0 && i < rq.tokens;
+    padding = rq.length < 0;
+  }
+  const int64_t cap = int64_t(g.columns) * g.page_size;
+  int64_t keys = int64_t(rq.length) + i + 1;
+  if (write && !padding) {
+    if (keys > cap) {
+      L = NAN;  // a token past the table
+    } else {
+      const int tq = 32 * p.own_qt;
+      const int64_t end = a.k ? keys : min(int64_t(rq.length) + min((i / tq + 1) * tq, rq.tokens), cap + 1);
+      splits = int((end + p.split_keys - 1) / p.split_keys);
+    }
+  }
+  const int pieces = splits ? p.pieces : 0;
+  float M = -INFINITY;
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  const float* base = p.partials + (int64_t(head) * a.rows + row) * part_row<DP>();
+  const int64_t step = int64_t(g.heads) * a.rows * part_row<DP>();
+#pragma unroll 4
+  for (int s = 0; s < pieces + splits; ++s) {
+    const float* x = base + s * step;
+    const float2 ml = *reinterpret_cast<const float2*>(x + DP);
+    const float4 v = *reinterpret_cast<const float4*>(x + dd);
+    const float top = fmaxf(M, ml.x);
+    const float wo = M == -INFINITY ? 0.f : fast_exp2(M - top);
+    const float wn = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    L = fmaf(L, wo, ml.y * wn);
+    if (isnan(ml.y)) L = NAN;
+    acc.x = fmaf(acc.x, wo, v.x * wn); acc.y = fmaf(acc.y, wo, v.y * wn);
+    acc.z = fmaf(acc.z, wo, v.z * wn); acc.w = fmaf(acc.w, wo, v.w * wn);
+    M = top;
+  }
+  T* const out = static_cast<T*>(a.out) + row * a.o_r + int64_t(head) * g.dim;
+  if (write && dd < g.dim)
+    store4<DT>(out + dd, finalize(acc.x, L), finalize(acc.y, L), finalize(acc.z, L), finalize(acc.w, L));
+  const float zero = fmaf(acc.x, 0.f, acc.y * 0.f) + fmaf(acc.z, 0.f, acc.w * 0.f);
+  uint64_t left = __ballot(write && isnan(zero) && !isnan(L));
+  while (left) {
+    const int first = __builtin_ctzll(left) / LANES * LANES;
+    left &= ~(((LANES == 64 ? 0 : uint64_t(1) << (LANES & 63)) - 1) << first);
+    const int64_t again = __shfl(row, first);
+    const int h = __shfl(head, first), req = __shfl(r, first);
+    const int64_t n = __shfl(keys, first);
+    const T* q = static_cast<const T*>(a.q) + again * a.q_r + int64_t(h) * g.dim;
+    const T* fk = a.k ? static_cast<const T*>(a.k) + again * a.q_r + int64_t(h) * g.dim : nullptr;
+    const T* fv = a.k ? static_cast<const T*>(a.v) + again * a.q_r + int64_t(h) * g.dim : nullptr;
+    Walk<DT> w;
+    w.keys(q, a.slabs, a.prefix_table, a.prefix_columns, 0, a.prefix, nullptr, nullptr, g, h, a.qscale);
+    w.keys(q, a.slabs, a.table + int64_t(req) * g.columns, g.columns, 0, n, fk, fv, g, h, a.qscale);
+    const float l = w.denominator();
+    T* const to = static_cast<T*>(a.out) + again * a.o_r + int64_t(h) * g.dim;
+    __threadfence_block();  // after the stores above, which it repeats
+    if (lane < g.dim) to[lane] = from_f32<DT>(finalize(w.acc[0], l));
+    if (lane + kWave < g.dim) to[lane + kWave] = from_f32<DT>(finalize(w.acc[1], l));
+  }
+}
+
 // ------------------------------------------------------------------- host ---
 bool shared_shape(int b, int rows, int max_tokens, int h, int d, int page_size, int pps, int num_slabs, int prefix,
                   int columns, int layer, int layers, int dtype) {
   return b > 0 && b <= 65535 && rows > 0 && max_tokens > 0 && max_tokens <= rows && h > 0 && d > 0 && d <= 128 &&
          int64_t(b) * h <= 65535 && int64_t(rows) * h * d <= INT32_MAX && (page_size == 8 || page_size == 16 || page_size == 32) &&
          pps > 0 && num_slabs > 0 && int64_t(pps) * num_slabs <= INT32_MAX && prefix >= 0 && columns > 0 &&
-         int64_t(b) * columns <= INT32_MAX && int64_t(columns) * page_size <= INT32_MAX &&
-         int64_t(prefix) + int64_t(columns) * page_size <= INT32_MAX && layers > 0 && layer >= 0 && layer < layers &&
+         int64_t(b) * columns <= INT32_MAX && int64_t(columns) * page_size <= INT32_MAX - 4096 &&
+         int64_t(prefix) <= INT32_MAX - 4096 - int64_t(columns) * page_size && layers > 0 && layer >= 0 && layer < layers &&
          dtype >= 0 && dtype <= 2;
 }
 
-hipError_t launch_shared(SharedArgs& a, int dtype) {
+int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
+
+// How a launch is cut.
+Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int columns, int max_tokens, int dtype, bool decode) {
+  const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
+  const int dp = d <= 64 ? 64 : 128, row_bytes = dp * (dtype == kF32 ? 4 : 2);
+  const int slots = (row_bytes == 128 ? 2 : 1) * cus;  // workgroups that are resident at once
+  const int64_t cap = int64_t(columns) * page_size, bh = int64_t(b) * h;
+  Plan p{};
+  // Prefix tiles: the queries' groups of 32 over tiles of 1, 2, 4 or 8 groups,
+  // where a tile costs its groups and about one more.
+  int64_t best = INT64_MAX;
+  for (int qt = 1; qt <= 8; qt *= 2) {
+    const int64_t cost = ceil_div(rows, 32 * qt) * (qt + 1);
+    if (cost <= best) { best = cost; p.qt = qt; }
+  }
+  p.tiles = int(ceil_div(rows, 32 * p.qt));
+  if (prefix > 0) {
+    const int64_t items = int64_t(p.tiles) * h;
+    const int64_t want = std::max<int64_t>(1, slots / items);
+    const int least = 64;  // keys of a piece
+    int64_t pieces = std::min<int64_t>(want, ceil_div(prefix, least));
+    pieces = std::max<int64_t>(pieces, ceil_div(prefix, kPages * page_size));
+    p.piece_keys = int(ceil_div(ceil_div(prefix, pieces), 32) * 32);
+    p.pieces = int(ceil_div(prefix, p.piece_keys));
+    p.prefix_items = items * p.pieces;
+  }
+  if (decode) {
+    const int waves = slots * kWaves;
+    p.item_waves = bh * 8 <= waves ? 8 : bh * 4 <= 2 * int64_t(waves) ? 4 : 2;
+    while (p.item_waves > 1 && (p.item_waves - 1) * 8 >= cap) p.item_waves /= 2;
+    // A wave resolves the page of each of its steps into one lane: 64 steps of 8 tokens.
+    const int64_t most = std::min<int64_t>(512 * p.item_waves, 2048);
+    const int64_t want = (cap * bh / slots + 63) / 64 * 64;
+    p.split_keys = int(std::min<int64_t>(most, std::max<int64_t>(want, 512)));
+    p.splits = int(ceil_div(cap, p.split_keys));
+    const int groups = kWaves / p.item_waves;
+    p.more_blocks = int(std::min<int64_t>(slots, (bh * (p.splits - 1) + groups - 1) / groups));
+    p.own_blocks = ceil_div(bh, groups);
+    p.own_qt = 1;
+  } else {
+    p.own_qt = max_tokens <= 32 ? 1 : max_tokens <= 64 ? 2 : 4;
+    p.own_tiles = int(ceil_div(max_tokens, 32 * p.own_qt));
+    p.split_keys = 2048;
+    p.splits = int(ceil_div(cap + 1, p.split_keys));
+    p.own_blocks = bh * p.own_tiles * p.splits;
+  }
+  return p;
+}
+
+// Whether one launch can hold the plan's workgroups.
+bool plan_fits(const Plan& p) { return p.prefix_items + p.own_blocks < (int64_t(1) << 30); }
+
+size_t plan_bytes(const Plan& p, int rows, int h, int d) {
+  return size_t(p.pieces + p.splits) * h * rows * (d <= 64 ? part_row<64>() : part_row<128>()) * sizeof(float);
+}
+
+// Rows that the fast path takes: whole 16-byte chunks.
+bool whole_chunks(int d, int dtype) { return d * (dtype == kF32 ? 4 : 2) % 16 == 0; }
+
+template <int DT, int DP>
+void launch_fast(const SharedArgs& a, const Plan& p) {
+  const int blocks = int(p.more_blocks + p.prefix_items + p.own_blocks);
+  if (!a.k) shared_kernel<DT, DP, kRowsFull, false><<<blocks, kThreads>>>(a, p);
+  else if (a.g.dim == DP) shared_kernel<DT, DP, kRowsFull, true><<<blocks, kThreads>>>(a, p);
+  else shared_kernel<DT, DP, kRowsPadded, true><<<blocks, kThreads>>>(a, p);
+  const int64_t pairs = int64_t(a.rows) * a.g.heads;
+  shared_merge_kernel<DT, DP><<<int(ceil_div(pairs, kMergeThreads / (DP / 4))), kMergeThreads>>>(a, p);
+}
+
+hipError_t launch_shared(SharedArgs& a, int dtype, void* workspace) {
+  const int es = dtype == kF32 ? 4 : 2;
+  auto rows16 = [&](int64_t x) { return x * es % 16 == 0; };
+  if (whole_chunks(a.g.dim, dtype) && rows16(a.q_r) && rows16(a.o_r) && aligned16(a.out) && aligned16(a.q) &&
+      (!a.k || (aligned16(a.k) && aligned16(a.v)))) {
+    Plan p = make_plan(a.rows, a.b, a.g.heads, a.g.dim, a.g.page_size, a.prefix, a.g.columns, a.max_tokens, dtype, a.k != nullptr);
+    p.partials = static_cast<float*>(workspace);
+#define MT_FAST(DT)                       \
+  if (a.g.dim <= 64) launch_fast<DT, 64>(a, p); \
+  else launch_fast<DT, 128>(a, p);
+    if (dtype == kF32) { MT_FAST(kF32) }
+    else if (dtype == kF16) { MT_FAST(kF16) }
+    else { MT_FAST(kBF16) }
+#undef MT_FAST
+    return hipGetLastError();
+  }
   const int64_t waves = int64_t(a.b) * a.max_tokens * a.g.heads;
   const int blocks = int(std::min<int64_t>((waves + 3) / 4, 1 << 20));
   if (dtype == kF32) shared_walk_kernel<kF32><<<blocks, 256>>>(a);
@@ -249,6 +1083,14 @@ int mt_paged_shared_workspace_bytes(int rows, int b, int h, int d, int page_size
   if (!bytes || !shared_shape(b, rows, max_tokens, h, d, page_size, 1, 1, prefix_tokens, columns, 0, 1, dtype))
     return hipErrorInvalidValue;
   *bytes = 0;
+  if (!whole_chunks(d, dtype)) return hipSuccess;
+  size_t need = 0;
+  for (int decode = 0; decode < (max_tokens == 1 && rows == b ? 2 : 1); ++decode) {
+    const Plan p = make_plan(rows, b, h, d, page_size, prefix_tokens, columns, max_tokens, dtype, decode);
+    if (!plan_fits(p)) return hipErrorInvalidValue;
+    need = std::max(need, plan_bytes(p, rows, h, d));
+  }
+  *bytes = need;
   return hipSuccess;
 }
 
@@ -272,7 +1114,7 @@ int mt_paged_shared_decode(void* out, const void* q, const void* k, const void* 
   a.qscale = (1.0f / std::sqrt(float(d))) * kLog2e;
   a.q_r = stride; a.o_r = hd;
   a.g = make_geometry(h, d, page_size, pages_per_slab, num_slabs, columns, layer);
-  return launch_shared(a, dtype);
+  return launch_shared(a, dtype, workspace);
 }
 
 int mt_paged_shared_attention(void* out, const void* q, const uint64_t* slabs, const int* prefix_table,
@@ -299,7 +1141,7 @@ int mt_paged_shared_attention(void* out, const void* q, const uint64_t* slabs, c
   a.qscale = (1.0f / std::sqrt(float(d))) * kLog2e;
   a.q_r = qs; a.o_r = os;
   a.g = make_geometry(h, d, page_size, pages_per_slab, num_slabs, columns, layer);
-  return launch_shared(a, dtype);
+  return launch_shared(a, dtype, workspace);
 }
 
 }  // extern "C"

@@ -97,6 +97,27 @@ def test_attention_refuses(bad):
     assert _call('shared_prefix_kernel', 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], ATTEND, bad) == 1
 
 
+@pytest.mark.parametrize('bad', [dict(workspace=None), dict(workspace=24), dict(size=0)])
+def test_attentions_refuse_a_workspace_that_does_not_do(bad):
+    lib = 'shared_prefix_kernel'
+    assert _call(lib, 'mt_paged_shared_decode', [P] * 8 + [I] * 12 + [P, Z], DECODE, bad) == 1
+    assert _call(lib, 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], ATTEND, bad) == 1
+
+
+def test_attention_refuses_more_workgroups_than_a_launch_has():
+    # 65535 requests that might each bring 2^20 tokens
+    big = dict(b=65535, rows=2 ** 24, max_tokens=2 ** 20, h=1, d=64, columns=2 ** 15)
+    assert _call('shared_prefix_kernel', 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], ATTEND, big) == 1
+
+
+def test_workspace_grows_with_the_batch():
+    args = dict(h=12, d=64, page_size=16, prefix_tokens=2000, columns=8, dtype='float16')
+    sizes = [paged_ops.shared_workspace_bytes(rows=b, b=b, max_tokens=1, **args) for b in (1, 8, 64)]
+    assert 0 < sizes[0] < sizes[1] < sizes[2]
+    # rows that are not whole 16-byte chunks use none
+    assert paged_ops.shared_workspace_bytes(rows=8, b=8, max_tokens=1, **dict(args, d=63)) == 0
+
+
 def test_python_reports_a_refusal():
     with pytest.raises(RuntimeError):
         paged_ops.paged_append_slots(16, 16, 16, 16, rows=0, h=12, d=64, page_size=16, pages_per_slab=4, num_slabs=8,
