@@ -212,6 +212,21 @@ constexpr int kPages = 512;  // pages of an item's keys, resolved into LDS
 constexpr float kRescale = 6.f;
 constexpr float kHalfShift = 9.f;  // 2^(kRescale + kHalfShift) is below fp16's largest
 
+// Small pools' slab tables are copied to LDS while the first table entries are on
+// their way, so that a page is one round trip away instead of two.
+constexpr int kLdsSlabs = 512;
+static_assert(kLdsSlabs <= kThreads, "a slab per thread");
+
+__device__ __forceinline__ uint64_t slab_entry(const SharedArgs& a) {
+  return a.g.num_slabs <= kLdsSlabs && int(threadIdx.x) < a.g.num_slabs ? a.slabs[threadIdx.x] : 0;
+}
+template <class T>
+__device__ __forceinline__ const T* page_of(const SharedArgs& a, const uint64_t* s_slabs, int physical, int head) {
+  if (!physical_in_pool(physical, a.g)) return nullptr;
+  const int slab = slab_index(physical, a.g);
+  return page_in_slab<T>(a.g.num_slabs <= kLdsSlabs ? s_slabs[slab] : a.slabs[slab], physical, a.g, head);
+}
+
 // How the launch is cut (made on the host).
 struct Plan {
   // prefix: tiles of 32 qt queries, pieces of piece_keys keys (a multiple of 32)
@@ -268,6 +283,34 @@ struct Shape {
   }
 };
 
+// Two weights as the high and low packed MFMA operands: hi rounded to the type
+// (fp16 toward zero, bf16 to nearest even), lo the remainder, rounded the same
+// way. The remainder, exact in fp32, takes one instruction a weight: a dot
+// product of the pair with (-1, 0) or (0, -1), added to it.
+template <int DT>
+__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  if constexpr (DT == kF16) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+    const h2 first = {-1, 0}, second = {0, -1};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_fdot2(h, first, p0, false),
+                                                                 __builtin_amdgcn_fdot2(h, second, p1, false)));
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 h = {static_cast<__bf16>(p0), static_cast<__bf16>(p1)};
+    // in registers: as an inline constant of this instruction -1.0 is the pair
+    // (0, -1), where the compiler takes it for (-1, 0)
+    uint32_t first = 0xBF80u, second = 0xBF800000u;
+    asm("" : "+s"(first));
+    asm("" : "+s"(second));
+    hi = __builtin_bit_cast(uint32_t, h);
+    const b2 r = {static_cast<__bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(b2, first), p0, false)),
+                  static_cast<__bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(b2, second), p1, false))};
+    lo = __builtin_bit_cast(uint32_t, r);
+  }
+}
+
 // A tile of queries and the keys [k0, k1) of a table row that it attends (k0 a
 // multiple of 32, at most kPages pages): query j those up to limit + j.
 struct Tile {
@@ -289,7 +332,7 @@ struct Tile {
 // it by kRescale only.
 template <int DT, int DP>
 __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, int head, char* s_raw,
-                                            typename Elem<DT>::T const** s_page, int* s_missing) {
+                                            typename Elem<DT>::T const** s_page, uint64_t* s_slabs, int* s_missing) {
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP>;
   constexpr int EC = S::EC, CPR = S::CPR, NC = S::NC, DT32 = S::DT32, QW = S::QW;
@@ -316,14 +359,18 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     qv[s] = *global_view(reinterpret_cast<const u32x4*>(p < chunks ? qrow + p * EC : reinterpret_cast<const T*>(g_fill + 4)));
   }
 
-  // the pages of the keys
+  // the pages of the keys, one a thread
+  static_assert(kPages <= kThreads, "a page per thread");
   const int pages = (t.k1 - t.k0 + g.page_size - 1) >> g.log2_page;
+  const int column = (t.k0 >> g.log2_page) + tid;
+  const int physical = tid < pages && column < t.columns ? t.table_row[column] : -1;
+  const uint64_t slab = slab_entry(a);
   if (tid == 0) *s_missing = 0;
+  if (tid < kLdsSlabs) s_slabs[tid] = slab;
   __syncthreads();
-  for (int j = tid; j < pages; j += kThreads) {
-    const int column = (t.k0 >> g.log2_page) + j;
-    const T* page = column < t.columns ? resolve_page<T>(a.slabs, t.table_row[column], g, head) : nullptr;
-    s_page[j] = page;
+  if (tid < pages) {
+    const T* page = page_of<T>(a, s_slabs, physical, head);
+    s_page[tid] = page;
     if (!page) *s_missing = 1;
   }
   __syncthreads();
@@ -416,8 +463,11 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     if (base + 31 > t.limit + q0 || base + 32 > t.k1) {
       const int last = last_key - base - 4 * grp;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (8 * (i >> 2) + (i & 3) > last) sc[i] = -INFINITY;
+      for (int i = 0; i < 16; ++i) {
+        float x = 8 * (i >> 2) + (i & 3) > last ? -INFINITY : sc[i];
+        asm volatile("" : "+v"(x));  // keeps this a branch: 46 instructions of a block's 190 without it
+        sc[i] = x;
+      }
     }
     float top = sc[0];
 #pragma unroll
@@ -473,7 +523,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t h2, l2;
-          SplitP<DT>::split(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
+          split_weights<DT>(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
           hi[w] = h2;
           lo[w] = l2;
         }
@@ -579,9 +629,11 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
 // lanes a token, U steps in flight; item_waves waves share an item. The keys of
 // split `split` of row `row`; the last split appends and scores the new token.
 // All threads of the workgroup enter (barriers); `on` where the group has an item.
+// What does not depend on the row's length -- table entries, query, new token --
+// is loaded with it, in one round trip.
 template <int DT, int DP, Rows FULL>
 __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, bool on, int row, int head, int split,
-                                            float* s_state) {
+                                            float* s_state, uint64_t* s_slabs, bool& slabs_there) {
   using T = typename Elem<DT>::T;
   constexpr int G = 8, DL = DP / G, RB = kWave / G;
   constexpr int U = DL * elem_bytes<DT>() >= 64 ? 1 : DL * elem_bytes<DT>() >= 32 ? 2 : 4;
@@ -591,104 +643,113 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & (kWave - 1);
   const int W = p.item_waves, gw = wave % W, first_wave = wave - gw;
   const int col0 = C::first_col(lane % G), tok = lane / G;
+  const int t0 = split * p.split_keys;
+  const int rel0 = (gw + W * lane) * RB;  // lane i: this wave's step i
+  const int* const table_row = a.table + int64_t(row) * g.columns;
+  const int64_t qrow = int64_t(row) * a.q_r + int64_t(head) * dim;
+  const int64_t column0 = (int64_t(t0) + rel0) >> g.log2_page;
+  int physical = -1, offset = -1;
+  Query<DT, DP, FULL, G> qv;
+  C kn, vn;
+  if (on) {
+    offset = a.lengths[row];
+    if (rel0 < p.split_keys && column0 < g.columns) physical = table_row[column0];
+    qv.load(static_cast<const T*>(a.q) + qrow, col0, dim, a.qscale);
+    if (gw == 0) {
+      kn.load(static_cast<const T*>(a.k) + qrow + col0, col0, dim);
+      vn.load(static_cast<const T*>(a.v) + qrow + col0, col0, dim);
+    }
+  }
+  if (!slabs_there) {
+    const uint64_t slab = slab_entry(a);
+    if (tid < kLdsSlabs) s_slabs[tid] = slab;
+    __syncthreads();
+    slabs_there = true;
+  }
+  const int64_t L = int64_t(offset) + 1;
+  on = offset >= 0 && L <= int64_t(g.columns) * g.page_size;
+  const int nsplit = on ? int((uint32_t(L) + uint32_t(p.split_keys) - 1) / uint32_t(p.split_keys)) : 0;
+  on = split < nsplit;
   Softmax<DL, G> st;
   st.init();
-  int nsplit = 1;
   if (on) {
-    const int offset = a.lengths[row];
-    const int64_t L = int64_t(offset) + 1, cap = int64_t(g.columns) * g.page_size;
-    on = offset >= 0 && L <= cap;
-    if (on) nsplit = int((uint32_t(L) + uint32_t(p.split_keys) - 1) / uint32_t(p.split_keys));
-    on = on && split < nsplit;
-    if (on) {
-      const int t0 = split * p.split_keys, t1 = int(L < int64_t(t0) + p.split_keys ? L : int64_t(t0) + p.split_keys);
-      const bool owns_new = split == nsplit - 1;
-      const int ntok = (owns_new ? t1 - 1 : t1) - t0;
-      const int* table_row = a.table + int64_t(row) * g.columns;
-      const int64_t qrow = int64_t(row) * a.q_r + int64_t(head) * dim;
-      Query<DT, DP, FULL, G> qv;
-      qv.load(static_cast<const T*>(a.q) + qrow, col0, dim, a.qscale);
-      // lane i: the page of this wave's step i
-      const int rel0 = (gw + W * lane) * RB;
-      const T* page = nullptr;
-      if (rel0 < ntok) page = resolve_page<T>(a.slabs, table_row[(t0 + rel0) >> g.log2_page], g, head);
-      const uint64_t at = reinterpret_cast<uintptr_t>(page);
-      const int at_lo = int(uint32_t(at)), at_hi = int(uint32_t(at >> 32));
-      const int steps_all = (ntok + RB - 1) / RB;
-      const int steps = steps_all > gw ? (steps_all - gw + W - 1) / W : 0;
-      for (int i0 = 0; i0 < steps; i0 += U) {
-        C kc[U], vc[U];
-        bool valid[U];
+    const int t1 = int(L < int64_t(t0) + p.split_keys ? L : int64_t(t0) + p.split_keys);
+    const bool owns_new = split == nsplit - 1;
+    const int ntok = (owns_new ? t1 - 1 : t1) - t0;
+    const int new_physical = owns_new && gw == 0 ? table_row[(t1 - 1) >> g.log2_page] : -1;
+    const T* page = rel0 < ntok ? page_of<T>(a, s_slabs, physical, head) : nullptr;
+    const uint64_t at = reinterpret_cast<uintptr_t>(page);
+    const int at_lo = int(uint32_t(at)), at_hi = int(uint32_t(at >> 32));
+    const int steps_all = (ntok + RB - 1) / RB;
+    const int steps = steps_all > gw ? (steps_all - gw + W - 1) / W : 0;
+    for (int i0 = 0; i0 < steps; i0 += U) {
+      C kc[U], vc[U];
+      bool valid[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = min(i0 + u, kWave - 1);
-          const int rel = (gw + W * (i0 + u)) * RB + tok;
-          valid[u] = rel < ntok;
-          const T* base = reinterpret_cast<const T*>(uint64_t(uint32_t(__builtin_amdgcn_readlane(at_hi, i))) << 32 |
-                                                     uint32_t(__builtin_amdgcn_readlane(at_lo, i)));
-          if (valid[u] && base) {
-            const T* kp = base + ((t0 + rel) & (g.page_size - 1)) * dim + col0;
-            kc[u].template load<true>(kp, col0, dim);
-            vc[u].template load<true>(kp + g.kind_stride, col0, dim);
-          } else {
-            kc[u].nan_fill();
-            vc[u].nan_fill();
-          }
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u, kWave - 1);
+        const int rel = (gw + W * (i0 + u)) * RB + tok;
+        valid[u] = rel < ntok;
+        const T* base = reinterpret_cast<const T*>(uint64_t(uint32_t(__builtin_amdgcn_readlane(at_hi, i))) << 32 |
+                                                   uint32_t(__builtin_amdgcn_readlane(at_lo, i)));
+        if (valid[u] && base) {
+          const T* kp = base + ((t0 + rel) & (g.page_size - 1)) * dim + col0;
+          kc[u].template load<true>(kp, col0, dim);
+          vc[u].template load<true>(kp + g.kind_stride, col0, dim);
+        } else {
+          kc[u].nan_fill();
+          vc[u].nan_fill();
         }
-        float s[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) s[u] = qv.score(kc[u]);
-        // one move of the running maximum for the U tokens; no scores but -Inf leave it
-        float top = st.m;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (valid[u]) top = fmaxf(top, s[u]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float alpha = fast_exp2(st.m - ref);
-        st.l *= alpha;
-#pragma unroll
-        for (int e = 0; e < DL; ++e) st.acc[e] *= alpha;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (!valid[u]) continue;
-          const float w = fast_exp2(s[u] - ref);
-          float vf[DL];
-          vc[u].to_float(vf);
-          st.l += w;
-#pragma unroll
-          for (int e = 0; e < DL; ++e) st.acc[e] = fmaf(w, vf[e], st.acc[e]);
-        }
-        st.m = top;
       }
-      if (owns_new && gw == 0) {
-        // the new token, by the first eight lanes: written to its page and scored
-        const int last = t1 - 1;
-        const T* np = resolve_page<T>(a.slabs, table_row[last >> g.log2_page], g, head);
-        C kn, vn;
-        kn.load(static_cast<const T*>(a.k) + qrow + col0, col0, dim);
-        vn.load(static_cast<const T*>(a.v) + qrow + col0, col0, dim);
-        if (np && lane < G) {
-          T* kp = const_cast<T*>(np) + (last & (g.page_size - 1)) * dim + col0;
-          T* vp = kp + g.kind_stride;
+      float s[U];
 #pragma unroll
-          for (int i = 0; i < C::NV; ++i) {
-            if (FULL == kRowsPadded && col0 + i * G * per16<DT>() >= dim) break;
-            global_view(reinterpret_cast<u32x4*>(kp))[i * G] = kn.raw[i];
-            global_view(reinterpret_cast<u32x4*>(vp))[i * G] = vn.raw[i];
-          }
-        }
-        if (!np) { kn.nan_fill(); vn.nan_fill(); }
-        const float sc = qv.score(kn);
-        if (lane < G) {
-          float vf[DL];
-          vn.to_float(vf);
-          const float top = fmaxf(st.m, sc), ref = top == -INFINITY ? 0.f : top;
-          const float alpha = fast_exp2(st.m - ref), w = fast_exp2(sc - ref);
-          st.l = fmaf(st.l, alpha, w);
+      for (int u = 0; u < U; ++u) s[u] = qv.score(kc[u]);
+      // one move of the running maximum for the U tokens; no scores but -Inf leave it
+      float top = st.m;
 #pragma unroll
-          for (int e = 0; e < DL; ++e) st.acc[e] = fmaf(w, vf[e], st.acc[e] * alpha);
-          st.m = top;
+      for (int u = 0; u < U; ++u)
+        if (valid[u]) top = fmaxf(top, s[u]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float alpha = fast_exp2(st.m - ref);
+      st.l *= alpha;
+#pragma unroll
+      for (int e = 0; e < DL; ++e) st.acc[e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!valid[u]) continue;
+        const float w = fast_exp2(s[u] - ref);
+        float vf[DL];
+        vc[u].to_float(vf);
+        st.l += w;
+#pragma unroll
+        for (int e = 0; e < DL; ++e) st.acc[e] = fmaf(w, vf[e], st.acc[e]);
+      }
+      st.m = top;
+    }
+    if (owns_new && gw == 0) {
+      // the new token, by the first eight lanes: written to its page and scored
+      const T* np = page_of<T>(a, s_slabs, new_physical, head);
+      if (np && lane < G) {
+        T* kp = const_cast<T*>(np) + ((t1 - 1) & (g.page_size - 1)) * dim + col0;
+        T* vp = kp + g.kind_stride;
+#pragma unroll
+        for (int i = 0; i < C::NV; ++i) {
+          if (FULL == kRowsPadded && col0 + i * G * per16<DT>() >= dim) break;
+          global_view(reinterpret_cast<u32x4*>(kp))[i * G] = kn.raw[i];
+          global_view(reinterpret_cast<u32x4*>(vp))[i * G] = vn.raw[i];
         }
+      }
+      if (!np) { kn.nan_fill(); vn.nan_fill(); }
+      const float sc = qv.score(kn);
+      if (lane < G) {
+        float vf[DL];
+        vn.to_float(vf);
+        const float top = fmaxf(st.m, sc), ref = top == -INFINITY ? 0.f : top;
+        const float alpha = fast_exp2(st.m - ref), w = fast_exp2(sc - ref);
+        st.l = fmaf(st.l, alpha, w);
+#pragma unroll
+        for (int e = 0; e < DL; ++e) st.acc[e] = fmaf(w, vf[e], st.acc[e] * alpha);
+        st.m = top;
       }
     }
   }
@@ -725,10 +786,12 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
 // Splits past the first of a decode's long rows: every workgroup counts them (rows
 // in chunks of a thread each) and takes its share, eight waves at a time.
 template <int DT, int DP, Rows FULL>
-__device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, int block, float* s_state, int* s_count) {
+__device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, int block, float* s_state, uint64_t* s_slabs,
+                                            int* s_count) {
   const Geometry& g = a.g;
   const int tid = threadIdx.x, groups = kWaves / p.item_waves, group = (tid >> 6) / p.item_waves;
   const int64_t cap = int64_t(g.columns) * g.page_size;
+  bool slabs_there = false;
   int64_t set = block;  // this workgroup's next set of `groups` items, less those of the chunks before
   for (int r0 = 0; r0 < a.b; r0 += kThreads) {
     int more = 0;
@@ -755,7 +818,7 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
       for (int step = kThreads / 2; step > 0; step >>= 1)
         if (s_count[i + step - 1] <= x) i += step;
       const int before = i ? s_count[i - 1] : 0;
-      stream_item<DT, DP, FULL>(a, p, on, r0 + i, head, 1 + x - before, s_state);
+      stream_item<DT, DP, FULL>(a, p, on, on ? r0 + i : 0, head, 1 + x - before, s_state, s_slabs, slabs_there);
     }
     set -= sets;
   }
@@ -775,13 +838,14 @@ void shared_kernel(SharedArgs a, Plan p) {
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP>;
   __shared__ const T* s_page[kPages];
+  __shared__ uint64_t s_slabs[kLdsSlabs];
   __shared__ int s_missing;
   __shared__ __align__(16) char s_raw[S::kLds];
   const Geometry& g = a.g;
   int block = int(blockIdx.x);
   if constexpr (DECODE) {
     if (block < p.more_blocks) {
-      stream_more<DT, DP, FULL>(a, p, block, reinterpret_cast<float*>(s_raw), reinterpret_cast<int*>(s_page));
+      stream_more<DT, DP, FULL>(a, p, block, reinterpret_cast<float*>(s_raw), s_slabs, reinterpret_cast<int*>(s_page));
       return;
     }
     block -= p.more_blocks;
@@ -802,7 +866,7 @@ void shared_kernel(SharedArgs a, Plan p) {
     t.k1 = min(a.prefix, t.k0 + p.piece_keys);
     t.limit = INT_MAX;
     t.part = part_of<DP>(a, p, piece, head, row);
-    attend_tile<DT, DP>(a, t, head, s_raw, s_page, &s_missing);
+    attend_tile<DT, DP>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
     return;
   }
   if constexpr (DECODE) {
@@ -810,7 +874,9 @@ void shared_kernel(SharedArgs a, Plan p) {
     const int64_t item = int64_t(index) * groups + (threadIdx.x >> 6) / p.item_waves;
     const bool on = item < int64_t(a.b) * g.heads;
     const int row = on ? int(item / g.heads) : 0;
-    stream_item<DT, DP, FULL>(a, p, on, row, int(item - int64_t(row) * g.heads), 0, reinterpret_cast<float*>(s_raw));
+    bool slabs_there = false;
+    stream_item<DT, DP, FULL>(a, p, on, row, on ? int(item - int64_t(row) * g.heads) : 0, 0,
+                              reinterpret_cast<float*>(s_raw), s_slabs, slabs_there);
   } else {
     // (split, request, tile, head)
     int i = index / g.heads;
@@ -835,26 +901,56 @@ void shared_kernel(SharedArgs a, Plan p) {
     t.k1 = int(min(end, k0 + p.split_keys));
     t.limit = int64_t(rq.length) + q0;
     t.part = part_of<DP>(a, p, p.pieces + split, head, row);
-    attend_tile<DT, DP>(a, t, head, s_raw, s_page, &s_missing);
+    attend_tile<DT, DP>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
   }
 }
 
-// Joins the pieces of every query: DP / 4 lanes a (row, head), four dims each. A
+// Joins the pieces of every query: DP / 4 lanes hold four dims each of a (row,
+// head), SUB groups of them every SUB-th piece. The prefix pieces are on their way
+// before the row's length is known. A
 // query left non-finite, and not by a missing page (whose NaN is the
-// denominator's too), is attended once more by a wave on the VALU: on the matrix
+// denominator's too), is attended once more by its wave on the VALU: on the matrix
 // cores a key that a query does not attend has weight 0, and 0 * Inf or 0 * NaN of
 // its V is NaN, and so is the 0 * Inf of a weight's low part.
 constexpr int kMergeThreads = 256;
-template <int DT, int DP>
+constexpr int kManyPieces = 8;  // from here on several groups of lanes share a (row, head)
+
+// Pieces joined so far: four dims of the accumulators, maximum, denominator.
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float2 ml, const float4& v) {
+    const float top = fmaxf(m, ml.x);
+    const float wo = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    const float wn = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    l = fmaf(l, wo, ml.y * wn);  // a NaN denominator stays
+    acc.x = fmaf(acc.x, wo, v.x * wn); acc.y = fmaf(acc.y, wo, v.y * wn);
+    acc.z = fmaf(acc.z, wo, v.z * wn); acc.w = fmaf(acc.w, wo, v.w * wn);
+    m = top;
+  }
+};
+
+template <int DT, int DP, int SUB>
 __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedArgs a, Plan p) {
   using T = typename Elem<DT>::T;
-  constexpr int LANES = DP / 4, PER = kMergeThreads / LANES;  // (row, head) pairs a workgroup
+  constexpr int LANES = DP / 4, PER = kMergeThreads / (LANES * SUB);  // pairs a workgroup
   __shared__ int s_count[kMergeThreads / kWave];
   const Geometry& g = a.g;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1);
-  const int64_t pair0 = int64_t(blockIdx.x) * PER, pair = pair0 + tid / LANES;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  const int64_t pair0 = int64_t(blockIdx.x) * PER, pair = pair0 + tid / (LANES * SUB);
   const int64_t row = pair / g.heads;
-  const int head = int(pair - row * g.heads), dd = 4 * (tid % LANES);
+  const int head = int(pair - row * g.heads), dd = 4 * (lane % LANES), sub = lane / LANES % SUB;
+  const float* base = p.partials + (int64_t(head) * a.rows + row) * part_row<DP>();
+  const int64_t step = int64_t(g.heads) * a.rows * part_row<DP>();
+  Joined all;
+  auto join = [&](int first, int end) {
+#pragma unroll 4
+    for (int s = first + sub; s < end; s += SUB) {
+      const float* x = base + s * step;
+      all.add(*reinterpret_cast<const float2*>(x + DP), *reinterpret_cast<const float4*>(x + dd));
+    }
+  };
+  if (row < a.rows) join(0, p.pieces);
   int r = int(row);
   if (a.cu_tokens) {
     // the request of the workgroup's first row: as many as start at or before it,
@@ -864,7 +960,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedArgs 
     for (int j = tid; j < a.b; j += kMergeThreads) n += a.cu_tokens[j] <= row0;
 #pragma unroll
     for (int w = kWave / 2; w > 0; w /= 2) n += __shfl_xor(n, w);
-    if (lane == 0) s_count[tid >> 6] = n;
+    if (lane == 0) s_count[wave] = n;
     __syncthreads();
     n = 0;
     for (int w = 0; w < kMergeThreads / kWave; ++w) n += s_count[w];
@@ -878,58 +974,43 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedArgs 
       }
     }
   }
-  // what the row attends; own keys in `splits` pieces
-  bool write = row < a.rows, padding = false;
-  int splits = 0, i = 0;
+  // what the row attends: nothing where it is no request's (`write` false)
   Request rq{0, 0, 0};
-  float L = 0.f;
-  if (write) {
-    rq = request_of(a, r);
-    i = int(row - rq.row0);
-    write = row >= rq.row0 && i < rq.tokens;
-    padding = rq.length < 0;
-  }
-  const int64_t cap = int64_t(g.columns) * g.page_size;
-  int64_t keys = int64_t(rq.length) + i + 1;
-  if (write && !padding) {
-    if (keys > cap) {
-      L = NAN;  // a token past the table
-    } else {
-      const int tq = 32 * p.own_qt;
-      const int64_t end = a.k ? keys : min(int64_t(rq.length) + min((i / tq + 1) * tq, rq.tokens), cap + 1);
-      splits = int((end + p.split_keys - 1) / p.split_keys);
+  if (row < a.rows) rq = request_of(a, r);
+  const int i = int(row - rq.row0);
+  const bool write = row < a.rows && row >= rq.row0 && i < rq.tokens;
+  const int64_t keys = int64_t(rq.length) + i + 1, cap = int64_t(g.columns) * g.page_size;
+  T* const out = static_cast<T*>(a.out) + row * a.o_r + int64_t(head) * g.dim;
+  bool redo = false;
+  if (write && (rq.length < 0 || keys > cap)) {
+    // padding, or a token past the table
+    if (sub == 0 && dd < g.dim) {
+      const float x = rq.length < 0 ? 0.f : NAN;
+      store4<DT>(out + dd, x, x, x, x);
+    }
+  } else if (write) {
+    const int tq = 32 * p.own_qt;
+    const int64_t end = a.k ? keys : min(int64_t(rq.length) + min((i / tq + 1) * tq, rq.tokens), cap + 1);
+    join(p.pieces, p.pieces + int((end + p.split_keys - 1) / p.split_keys));
+#pragma unroll
+    for (int w = LANES; w < LANES * SUB; w <<= 1)
+      all.add(float2{__shfl_xor(all.m, w), __shfl_xor(all.l, w)},
+              float4{__shfl_xor(all.acc.x, w), __shfl_xor(all.acc.y, w), __shfl_xor(all.acc.z, w), __shfl_xor(all.acc.w, w)});
+    const float zero = fmaf(all.acc.x, 0.f, all.acc.y * 0.f) + fmaf(all.acc.z, 0.f, all.acc.w * 0.f);
+    redo = isnan(zero) && !isnan(all.l);
+    if (sub == 0 && dd < g.dim) {
+      const float inv = inverse(all.l);
+      store4<DT>(out + dd, divided<DT>(all.acc.x, all.l, inv), divided<DT>(all.acc.y, all.l, inv),
+                 divided<DT>(all.acc.z, all.l, inv), divided<DT>(all.acc.w, all.l, inv));
     }
   }
-  const int pieces = splits ? p.pieces : 0;
-  float M = -INFINITY;
-  float4 acc = {0.f, 0.f, 0.f, 0.f};
-  const float* base = p.partials + (int64_t(head) * a.rows + row) * part_row<DP>();
-  const int64_t step = int64_t(g.heads) * a.rows * part_row<DP>();
-#pragma unroll 4
-  for (int s = 0; s < pieces + splits; ++s) {
-    const float* x = base + s * step;
-    const float2 ml = *reinterpret_cast<const float2*>(x + DP);
-    const float4 v = *reinterpret_cast<const float4*>(x + dd);
-    const float top = fmaxf(M, ml.x);
-    const float wo = M == -INFINITY ? 0.f : fast_exp2(M - top);
-    const float wn = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-    L = fmaf(L, wo, ml.y * wn);
-    if (isnan(ml.y)) L = NAN;
-    acc.x = fmaf(acc.x, wo, v.x * wn); acc.y = fmaf(acc.y, wo, v.y * wn);
-    acc.z = fmaf(acc.z, wo, v.z * wn); acc.w = fmaf(acc.w, wo, v.w * wn);
-    M = top;
-  }
-  T* const out = static_cast<T*>(a.out) + row * a.o_r + int64_t(head) * g.dim;
-  if (write && dd < g.dim)
-    store4<DT>(out + dd, finalize(acc.x, L), finalize(acc.y, L), finalize(acc.z, L), finalize(acc.w, L));
-  const float zero = fmaf(acc.x, 0.f, acc.y * 0.f) + fmaf(acc.z, 0.f, acc.w * 0.f);
-  uint64_t left = __ballot(write && isnan(zero) && !isnan(L));
+  uint64_t left = __ballot(redo);
+  if (left) __threadfence_block();  // the stores above come before those that repeat them
   while (left) {
-    const int first = __builtin_ctzll(left) / LANES * LANES;
-    left &= ~(((LANES == 64 ? 0 : uint64_t(1) << (LANES & 63)) - 1) << first);
-    const int64_t again = __shfl(row, first);
+    const int first = __builtin_ctzll(left) / (LANES * SUB) * (LANES * SUB);
+    left &= LANES * SUB == kWave ? 0 : ~(((uint64_t(1) << (LANES * SUB & 63)) - 1) << first);
+    const int64_t again = __shfl(row, first), n = __shfl(keys, first);
     const int h = __shfl(head, first), req = __shfl(r, first);
-    const int64_t n = __shfl(keys, first);
     const T* q = static_cast<const T*>(a.q) + again * a.q_r + int64_t(h) * g.dim;
     const T* fk = a.k ? static_cast<const T*>(a.k) + again * a.q_r + int64_t(h) * g.dim : nullptr;
     const T* fv = a.k ? static_cast<const T*>(a.v) + again * a.q_r + int64_t(h) * g.dim : nullptr;
@@ -938,7 +1019,6 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedArgs 
     w.keys(q, a.slabs, a.table + int64_t(req) * g.columns, g.columns, 0, n, fk, fv, g, h, a.qscale);
     const float l = w.denominator();
     T* const to = static_cast<T*>(a.out) + again * a.o_r + int64_t(h) * g.dim;
-    __threadfence_block();  // after the stores above, which it repeats
     if (lane < g.dim) to[lane] = from_f32<DT>(finalize(w.acc[0], l));
     if (lane + kWave < g.dim) to[lane + kWave] = from_f32<DT>(finalize(w.acc[1], l));
   }
@@ -1022,7 +1102,9 @@ void launch_fast(const SharedArgs& a, const Plan& p) {
   else if (a.g.dim == DP) shared_kernel<DT, DP, kRowsFull, true><<<blocks, kThreads>>>(a, p);
   else shared_kernel<DT, DP, kRowsPadded, true><<<blocks, kThreads>>>(a, p);
   const int64_t pairs = int64_t(a.rows) * a.g.heads;
-  shared_merge_kernel<DT, DP><<<int(ceil_div(pairs, kMergeThreads / (DP / 4))), kMergeThreads>>>(a, p);
+  constexpr int LANES = DP / 4;
+  if (p.pieces >= kManyPieces) shared_merge_kernel<DT, DP, kWave / LANES><<<int(ceil_div(pairs, kMergeThreads / kWave)), kMergeThreads>>>(a, p);
+  else shared_merge_kernel<DT, DP, 1><<<int(ceil_div(pairs, kMergeThreads / LANES)), kMergeThreads>>>(a, p);
 }
 
 hipError_t launch_shared(SharedArgs& a, int dtype, void* workspace) {
