@@ -283,32 +283,23 @@ struct Shape {
   }
 };
 
-// Two weights as the high and low packed MFMA operands: hi rounded to the type
-// (fp16 toward zero, bf16 to nearest even), lo the remainder, rounded the same
-// way. The remainder, exact in fp32, takes one instruction a weight: a dot
-// product of the pair with (-1, 0) or (0, -1), added to it.
-template <int DT>
-__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  if constexpr (DT == kF16) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-    const h2 first = {-1, 0}, second = {0, -1};
-    hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_fdot2(h, first, p0, false),
-                                                                 __builtin_amdgcn_fdot2(h, second, p1, false)));
-  } else {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 h = {static_cast<__bf16>(p0), static_cast<__bf16>(p1)};
-    // in registers: as an inline constant of this instruction -1.0 is the pair
-    // (0, -1), where the compiler takes it for (-1, 0)
-    uint32_t first = 0xBF80u, second = 0xBF800000u;
-    asm("" : "+s"(first));
-    asm("" : "+s"(second));
-    hi = __builtin_bit_cast(uint32_t, h);
-    const b2 r = {static_cast<__bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(b2, first), p0, false)),
-                  static_cast<__bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(b2, second), p1, false))};
-    lo = __builtin_bit_cast(uint32_t, r);
-  }
+// The largest of 16 scores (NaN ones are dropped), three a time in two chains; the
+// compiler's own maxima also pass every product through a maximum with itself. Its
+// first one stays: the compiler knows how long after the matrix product it may
+// read the scores, and the instructions written here wait for its result.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+__device__ __forceinline__ float largest(const floatx16& s) {
+  const float first = fmaxf(s[0], s[1]);
+  float x = max3(first, s[2], s[3]), y = max3(first, s[4], s[5]);
+  x = max3(x, s[6], s[7]);
+  y = max3(y, s[8], s[9]);
+  x = max3(x, s[10], s[11]);
+  y = max3(y, s[12], s[13]);
+  return max3(max3(x, s[14], s[15]), y, y);
 }
 
 // A tile of queries and the keys [k0, k1) of a table row that it attends (k0 a
@@ -417,6 +408,8 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
   };
 
   float m = -INFINITY, l = 0.f;
+  const float unscale = 1.f / a.qscale;
+  float threshold = -INFINITY;  // a product past it moves the reference
   floatx16 o[DT32];
 #pragma unroll
   for (int d = 0; d < DT32; ++d)
@@ -469,12 +462,10 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
         sc[i] = x;
       }
     }
-    float top = sc[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);  // NaN scores are dropped
-    top = max_halves(top) * a.qscale;
-    if (__any(top > m + kRescale)) {  // also a query's first keys, m = -inf
-      const float mn = fmaxf(m, top);
+    // (each lane asks for its own half of the keys; a query's first ones, m = -inf, too)
+    const float mine = largest(sc);
+    if (__any(mine > threshold)) {
+      const float mn = fmaxf(m, max_halves(mine) * a.qscale);
       const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
       l *= alpha;
 #pragma unroll
@@ -482,6 +473,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
       m = mn;
+      threshold = (m + kRescale) * unscale;
     }
     const float ref = m == -INFINITY ? 0.f : m - kShift;
 #pragma unroll
@@ -523,20 +515,24 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t h2, l2;
-          split_weights<DT>(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
+          SplitP<DT>::split(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
           hi[w] = h2;
           lo[w] = l2;
         }
+        u32x4 vt[DT32];
 #pragma unroll
         for (int d = 0; d < DT32; ++d) {
           const int rr = 4 * grp + (t16 >> 2);
           const int p = 4 * d + ((lane >> 4) & 1) * 2 + ((t16 & 3) >> 1);
           const T* v_at = s_v + (16 * s + rr) * DP + S::vpos(rr, p) * 8 + (t16 & 1) * 4;
           const uint2 x = read_transposed(v_at), y = read_transposed(v_at + 8 * DP);
-          const u32x4 vv = {x.x, x.y, y.x, y.y};
-          o[d] = mfma32<DT>(vv, hi, o[d]);
-          o[d] = mfma32<DT>(vv, lo, o[d]);
+          vt[d] = u32x4{x.x, x.y, y.x, y.y};
         }
+        // (no product waits for the one before it)
+#pragma unroll
+        for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], hi, o[d]);
+#pragma unroll
+        for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], lo, o[d]);
       }
     }
   };
