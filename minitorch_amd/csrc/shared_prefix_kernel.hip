@@ -206,8 +206,6 @@ __global__ __launch_bounds__(256) void shared_walk_kernel(SharedArgs a) {
 //     VALU, streaming (decode), several on the matrix cores, causally.
 // The first is bound by the matrix cores and the VALU between them, the second by
 // memory, so that one launch that mixes them runs both at once.
-constexpr int kWaves = 8;
-constexpr int kThreads = kWaves * kWave;
 constexpr int kPages = 512;  // pages of an item's keys, resolved into LDS
 constexpr float kRescale = 6.f;
 constexpr float kHalfShift = 9.f;  // 2^(kRescale + kHalfShift) is below fp16's largest
@@ -215,11 +213,22 @@ constexpr float kHalfShift = 9.f;  // 2^(kRescale + kHalfShift) is below fp16's 
 // Small pools' slab tables are copied to LDS while the first table entries are on
 // their way, so that a page is one round trip away instead of two.
 constexpr int kLdsSlabs = 512;
-static_assert(kLdsSlabs <= kThreads, "a slab per thread");
 
-__device__ __forceinline__ uint64_t slab_entry(const SharedArgs& a) {
-  return a.g.num_slabs <= kLdsSlabs && int(threadIdx.x) < a.g.num_slabs ? a.slabs[threadIdx.x] : 0;
-}
+template <int NT>
+struct SlabEntries {
+  uint64_t entry[kLdsSlabs / NT];
+  __device__ __forceinline__ void load(const SharedArgs& a) {
+#pragma unroll
+    for (int j = 0; j < kLdsSlabs / NT; ++j) {
+      const int i = int(threadIdx.x) + j * NT;
+      entry[j] = a.g.num_slabs <= kLdsSlabs && i < a.g.num_slabs ? a.slabs[i] : 0;
+    }
+  }
+  __device__ __forceinline__ void store(uint64_t* s_slabs) const {
+#pragma unroll
+    for (int j = 0; j < kLdsSlabs / NT; ++j) s_slabs[threadIdx.x + j * NT] = entry[j];
+  }
+};
 template <class T>
 __device__ __forceinline__ const T* page_of(const SharedArgs& a, const uint64_t* s_slabs, int physical, int head) {
   if (!physical_in_pool(physical, a.g)) return nullptr;
@@ -251,10 +260,14 @@ __device__ __forceinline__ float* part_of(const SharedArgs& a, const Plan& p, in
   return p.partials + ((int64_t(piece) * a.g.heads + head) * a.rows + row) * part_row<DP>();
 }
 
-// Staged keys of a workgroup of eight waves: two halves of kHalf keys, K and V
-// each. A wave takes blocks of 32 keys: with few waves per query group (KG <=
-// kHalf / 32) a round is one half, staged while the other is computed; with more,
-// both halves at once.
+// Waves of a workgroup: four where their operands take 256 registers a lane, so
+// that two workgroups still share a compute unit -- a prefix item and own ones
+// (rows of 512 bytes stay with eight, for the sake of their rounds).
+constexpr int shape_waves(int row_bytes) { return row_bytes == 256 ? 4 : 8; }
+
+// Staged keys of a workgroup: two halves of kHalf keys, K and V each. A wave takes
+// blocks of 32 keys: with few waves per query group (KG <= kHalf / 32) a round is
+// one half, staged while the other is computed; with more, both halves at once.
 template <int DT, int DP>
 struct Shape {
   static constexpr int ES = elem_bytes<DT>();
@@ -262,16 +275,18 @@ struct Shape {
   static constexpr int CPR = DP / EC;         // chunks per row
   static constexpr int RW = kWave / CPR;      // rows one load instruction of a wave fills
   static constexpr int kRowBytes = DP * ES;
-  static constexpr int kHalf = kRowBytes == 512 ? 64 : 128;
+  static constexpr int W = shape_waves(kRowBytes);
+  static constexpr int NT = W * kWave;
+  static constexpr int kHalf = kRowBytes == 128 ? 128 : 64;
   static constexpr int kBlocks = kHalf / 32;
   static constexpr int kPlane = kHalf * kRowBytes;
-  static constexpr int NC = kHalf / (kWaves * RW);  // loads per lane, K and V each
+  static constexpr int NC = kHalf / (W * RW);  // loads per lane, K and V each
   static constexpr int DT32 = DP / 32;
   static constexpr int QW = DT == kF32 ? DP / 8 : DP / 16;  // 16-byte query registers
   static constexpr int OS = DP + 4;
-  static constexpr size_t kMerge = size_t(kWaves) * 32 * (OS + 2) * sizeof(float);
+  static constexpr size_t kMerge = size_t(W) * 32 * (OS + 2) * sizeof(float);
   static constexpr size_t kLds = size_t(4) * kPlane > kMerge ? size_t(4) * kPlane : kMerge;
-  static constexpr int SW = kRowBytes == 128 ? 4 : 2;  // waves per SIMD: two workgroups a compute unit, or one
+  static constexpr int SW = kRowBytes == 128 ? 4 : 2;  // waves per SIMD: two workgroups a compute unit (512-byte rows: one)
   // Chunk p of key row r lies at chunk kpos / vpos of the row (both their own
   // inverse), so that the reads below are free of bank conflicts: K 16 bytes of
   // 32 consecutive rows, V 4 rows x 64 bytes (16-bit) or two rows 4 apart x 128
@@ -326,14 +341,14 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
                                             typename Elem<DT>::T const** s_page, uint64_t* s_slabs, int* s_missing) {
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP>;
-  constexpr int EC = S::EC, CPR = S::CPR, NC = S::NC, DT32 = S::DT32, QW = S::QW;
+  constexpr int EC = S::EC, CPR = S::CPR, NC = S::NC, DT32 = S::DT32, QW = S::QW, W = S::W, NT = S::NT;
   constexpr float kShift = DT == kF16 ? kHalfShift : 0.f;
   constexpr int CH = DP == 64 ? 4 : 2;  // chains of an fp32 block's sums
   const Geometry& g = a.g;
   const int dim = g.dim, chunks = dim / EC;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int qt_n = t.qt, kg_n = kWaves / qt_n;
+  const int qt_n = t.qt, kg_n = W / qt_n;
   const int kg = wave / qt_n, qt = wave - kg * qt_n;
   const int grp = lane >> 5, col = lane & 31;
   const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)s_raw));
@@ -350,18 +365,25 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     qv[s] = *global_view(reinterpret_cast<const u32x4*>(p < chunks ? qrow + p * EC : reinterpret_cast<const T*>(g_fill + 4)));
   }
 
-  // the pages of the keys, one a thread
-  static_assert(kPages <= kThreads, "a page per thread");
+  // the pages of the keys
   const int pages = (t.k1 - t.k0 + g.page_size - 1) >> g.log2_page;
-  const int column = (t.k0 >> g.log2_page) + tid;
-  const int physical = tid < pages && column < t.columns ? t.table_row[column] : -1;
-  const uint64_t slab = slab_entry(a);
+  int physical[kPages / NT];
+#pragma unroll
+  for (int j = 0; j < kPages / NT; ++j) {
+    const int i = tid + j * NT, column = (t.k0 >> g.log2_page) + i;
+    physical[j] = i < pages && column < t.columns ? t.table_row[column] : -1;
+  }
+  SlabEntries<NT> slabs;
+  slabs.load(a);
   if (tid == 0) *s_missing = 0;
-  if (tid < kLdsSlabs) s_slabs[tid] = slab;
+  slabs.store(s_slabs);
   __syncthreads();
-  if (tid < pages) {
-    const T* page = page_of<T>(a, s_slabs, physical, head);
-    s_page[tid] = page;
+#pragma unroll
+  for (int j = 0; j < kPages / NT; ++j) {
+    const int i = tid + j * NT;
+    if (i >= pages) break;
+    const T* page = page_of<T>(a, s_slabs, physical[j], head);
+    s_page[i] = page;
     if (!page) *s_missing = 1;
   }
   __syncthreads();
@@ -375,19 +397,19 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     if (plain && k + S::kHalf <= t.k1) {
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        const int r = sr + n * kWaves * S::RW;
+        const int r = sr + n * W * S::RW;
         const T* page = s_page[(k + r - t.k0) >> g.log2_page] + (r & (g.page_size - 1)) * dim;
-        stage16(page + S::kpos(r, spos) * EC, lk + n * kWaves * 1024);
-        stage16(page + g.kind_stride + S::vpos(r, spos) * EC, lv + n * kWaves * 1024);
+        stage16(page + S::kpos(r, spos) * EC, lk + n * W * 1024);
+        stage16(page + g.kind_stride + S::vpos(r, spos) * EC, lv + n * W * 1024);
       }
     } else {
       int row = sr;
       asm volatile("" : "+v"(row));  // keeps this rarer path's terms out of the registers of the loop
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        const int r = row + n * kWaves * S::RW, key = k + r;
+        const int r = row + n * W * S::RW, key = k + r;
         // a block wholly past the keys is never read
-        if (k + ((wave * S::RW + n * kWaves * S::RW) & ~31) >= t.k1) continue;
+        if (k + ((wave * S::RW + n * W * S::RW) & ~31) >= t.k1) continue;
         const int pk = S::kpos(r, spos), pv = S::vpos(r, spos);
         const T* kp = reinterpret_cast<const T*>(g_fill + 4);
         const T* vp = kp;
@@ -401,8 +423,8 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
             if (pv < chunks) vp = page + g.kind_stride + pv * EC;
           }
         }
-        stage16(kp, lk + n * kWaves * 1024);
-        stage16(vp, lv + n * kWaves * 1024);
+        stage16(kp, lk + n * W * 1024);
+        stage16(vp, lv + n * W * 1024);
       }
     }
   };
@@ -447,7 +469,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
         }
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = CH == 4 ? (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]) : part[0][i] + part[1][i];
+      for (int i = 0; i < 16; ++i) sc[i] = (part[0][i] + part[1][i]) + (CH == 4 ? part[CH - 2][i] + part[CH - 1][i] : 0.f);
     } else {
 #pragma unroll
       for (int s = 0; s < QW; ++s) sc = mfma32<DT>(read_k(s), qv[s], sc);
@@ -503,7 +525,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          o[d][i] += CH == 4 ? (ob[0][i] + ob[1][i]) + (ob[2][i] + ob[3][i]) : ob[0][i] + ob[1][i];
+          o[d][i] += (ob[0][i] + ob[1][i]) + (CH == 4 ? ob[CH - 2][i] + ob[CH - 1][i] : 0.f);
       }
     } else {
       // 16 keys a step: slot j < 4 of a lane holds key 16 s + 4 grp + j, slot j
@@ -589,7 +611,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     return;
   }
   float* const s_o = reinterpret_cast<float*>(s_raw);
-  float2* const s_ml = reinterpret_cast<float2*>(s_o + kWaves * 32 * S::OS);
+  float2* const s_ml = reinterpret_cast<float2*>(s_o + W * 32 * S::OS);
   const int tq = 32 * qt_n;
   __syncthreads();
   {
@@ -602,7 +624,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     if (grp == 0) s_ml[kg * tq + qi] = float2{m, l};
   }
   __syncthreads();
-  for (int u = tid; u < t.nq * (DP / 4); u += kThreads) {
+  for (int u = tid; u < t.nq * (DP / 4); u += NT) {
     const int q = u / (DP / 4), dd = 4 * (u - q * (DP / 4));
     float M = -INFINITY, L = 0.f;
     for (int k = 0; k < kg_n; ++k) M = fmaxf(M, s_ml[k * tq + q].x);
@@ -637,6 +659,7 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
   const Geometry& g = a.g;
   const int dim = FULL == kRowsFull ? DP : g.dim;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & (kWave - 1);
+  constexpr int WAVES = Shape<DT, DP>::W;
   const int W = p.item_waves, gw = wave % W, first_wave = wave - gw;
   const int col0 = C::first_col(lane % G), tok = lane / G;
   const int t0 = split * p.split_keys;
@@ -657,8 +680,9 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
     }
   }
   if (!slabs_there) {
-    const uint64_t slab = slab_entry(a);
-    if (tid < kLdsSlabs) s_slabs[tid] = slab;
+    SlabEntries<WAVES * kWave> slabs;
+    slabs.load(a);
+    slabs.store(s_slabs);
     __syncthreads();
     slabs_there = true;
   }
@@ -750,8 +774,8 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
     }
   }
   // States of the 16-lane rows by DPP, then the item's 4 W of them in LDS.
-  float* const s_acc = s_state;                            // [32][DP]
-  float2* const s_ml = reinterpret_cast<float2*>(s_state + 4 * kWaves * DP);
+  float* const s_acc = s_state;  // [4 WAVES][DP]
+  float2* const s_ml = reinterpret_cast<float2*>(s_state + 4 * WAVES * DP);
   st.row_merge();
   if ((lane & 15) < G) {
     const int si = wave * 4 + (lane >> 4);
@@ -780,16 +804,17 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
 }
 
 // Splits past the first of a decode's long rows: every workgroup counts them (rows
-// in chunks of a thread each) and takes its share, eight waves at a time.
+// in chunks of a thread each) and takes its share.
 template <int DT, int DP, Rows FULL>
 __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, int block, float* s_state, uint64_t* s_slabs,
                                             int* s_count) {
+  constexpr int WAVES = Shape<DT, DP>::W, NT = WAVES * kWave;
   const Geometry& g = a.g;
-  const int tid = threadIdx.x, groups = kWaves / p.item_waves, group = (tid >> 6) / p.item_waves;
+  const int tid = threadIdx.x, groups = WAVES / p.item_waves, group = (tid >> 6) / p.item_waves;
   const int64_t cap = int64_t(g.columns) * g.page_size;
   bool slabs_there = false;
   int64_t set = block;  // this workgroup's next set of `groups` items, less those of the chunks before
-  for (int r0 = 0; r0 < a.b; r0 += kThreads) {
+  for (int r0 = 0; r0 < a.b; r0 += NT) {
     int more = 0;
     if (r0 + tid < a.b) {
       const int64_t L = int64_t(a.lengths[r0 + tid]) + 1;
@@ -798,12 +823,12 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
     // inclusive sums over the chunk
     int sum = wave_inclusive_add(more);
     __syncthreads();
-    if ((tid & 63) == 63) s_count[kThreads + (tid >> 6)] = sum;
+    if ((tid & 63) == 63) s_count[NT + (tid >> 6)] = sum;
     __syncthreads();
-    for (int w = 0; w < (tid >> 6); ++w) sum += s_count[kThreads + w];
+    for (int w = 0; w < (tid >> 6); ++w) sum += s_count[NT + w];
     s_count[tid] = sum;
     __syncthreads();
-    const int64_t items = int64_t(s_count[kThreads - 1]) * g.heads;
+    const int64_t items = int64_t(s_count[NT - 1]) * g.heads;
     const int64_t sets = (items + groups - 1) / groups;
     for (; set < sets; set += p.more_blocks) {
       const int64_t item = set * groups + group;
@@ -811,7 +836,7 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
       const int x = on ? int(item / g.heads) : 0, head = on ? int(item - int64_t(x) * g.heads) : 0;
       int i = 0;  // the first row whose sum passes x
 #pragma unroll
-      for (int step = kThreads / 2; step > 0; step >>= 1)
+      for (int step = NT / 2; step > 0; step >>= 1)
         if (s_count[i + step - 1] <= x) i += step;
       const int before = i ? s_count[i - 1] : 0;
       stream_item<DT, DP, FULL>(a, p, on, on ? r0 + i : 0, head, 1 + x - before, s_state, s_slabs, slabs_there);
@@ -820,16 +845,8 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
   }
 }
 
-// Which item a workgroup works on: `count` of `all` workgroups are of the first
-// kind, spread evenly. Returns the index among its kind.
-__device__ __forceinline__ bool spread(int64_t block, int64_t count, int64_t all, int& index) {
-  const int64_t before = block * count / all, upto = (block + 1) * count / all;
-  index = int(upto > before ? before : block - before);
-  return upto > before;
-}
-
 template <int DT, int DP, Rows FULL, bool DECODE>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(Shape<DT, DP>::SW)))
+__global__ __launch_bounds__((Shape<DT, DP>::NT)) __attribute__((amdgpu_waves_per_eu((Shape<DT, DP>::SW))))
 void shared_kernel(SharedArgs a, Plan p) {
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP>;
@@ -838,16 +855,10 @@ void shared_kernel(SharedArgs a, Plan p) {
   __shared__ int s_missing;
   __shared__ __align__(16) char s_raw[S::kLds];
   const Geometry& g = a.g;
-  int block = int(blockIdx.x);
-  if constexpr (DECODE) {
-    if (block < p.more_blocks) {
-      stream_more<DT, DP, FULL>(a, p, block, reinterpret_cast<float*>(s_raw), s_slabs, reinterpret_cast<int*>(s_page));
-      return;
-    }
-    block -= p.more_blocks;
-  }
-  int index;
-  if (spread(block, p.prefix_items, p.prefix_items + p.own_blocks, index)) {
+  // The prefix items first: they are the long ones, at most one a compute unit
+  // where own items follow, which then take the rest of it.
+  int index = int(blockIdx.x);
+  if (index < p.prefix_items) {
     // (piece, head, tile), the tiles of a piece side by side
     const int ph = index / p.tiles, tile = index - ph * p.tiles;
     const int piece = ph / g.heads, head = ph - piece * g.heads;
@@ -865,8 +876,14 @@ void shared_kernel(SharedArgs a, Plan p) {
     attend_tile<DT, DP>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
     return;
   }
+  index -= int(p.prefix_items);
   if constexpr (DECODE) {
-    const int groups = kWaves / p.item_waves;
+    if (index < p.more_blocks) {
+      stream_more<DT, DP, FULL>(a, p, index, reinterpret_cast<float*>(s_raw), s_slabs, reinterpret_cast<int*>(s_page));
+      return;
+    }
+    index -= p.more_blocks;
+    const int groups = S::W / p.item_waves;
     const int64_t item = int64_t(index) * groups + (threadIdx.x >> 6) / p.item_waves;
     const bool on = item < int64_t(a.b) * g.heads;
     const int row = on ? int(item / g.heads) : 0;
@@ -1036,22 +1053,22 @@ int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 // How a launch is cut.
 Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int columns, int max_tokens, int dtype, bool decode) {
   const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
-  const int dp = d <= 64 ? 64 : 128, row_bytes = dp * (dtype == kF32 ? 4 : 2);
-  const int slots = (row_bytes == 128 ? 2 : 1) * cus;  // workgroups that are resident at once
+  const int row_bytes = (d <= 64 ? 64 : 128) * (dtype == kF32 ? 4 : 2), waves = shape_waves(row_bytes);
+  const int slots = (row_bytes == 512 ? 1 : 2) * cus;  // workgroups that are resident at once
   const int64_t cap = int64_t(columns) * page_size, bh = int64_t(b) * h;
   Plan p{};
   // Prefix tiles: the queries' groups of 32 over tiles of 1, 2, 4 or 8 groups,
   // where a tile costs its groups and about one more.
   int64_t best = INT64_MAX;
-  for (int qt = 1; qt <= 8; qt *= 2) {
+  for (int qt = 1; qt <= waves; qt *= 2) {
     const int64_t cost = ceil_div(rows, 32 * qt) * (qt + 1);
     if (cost <= best) { best = cost; p.qt = qt; }
   }
   p.tiles = int(ceil_div(rows, 32 * p.qt));
   if (prefix > 0) {
     const int64_t items = int64_t(p.tiles) * h;
-    const int64_t want = std::max<int64_t>(1, slots / items);
-    const int least = 64;  // keys of a piece
+    const int64_t want = std::max<int64_t>(1, cus / items);
+    const int least = items * ceil_div(prefix, 256) < cus / 4 ? 64 : 256;  // keys of a piece
     int64_t pieces = std::min<int64_t>(want, ceil_div(prefix, least));
     pieces = std::max<int64_t>(pieces, ceil_div(prefix, kPages * page_size));
     p.piece_keys = int(ceil_div(ceil_div(prefix, pieces), 32) * 32);
@@ -1059,20 +1076,21 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
     p.prefix_items = items * p.pieces;
   }
   if (decode) {
-    const int waves = slots * kWaves;
-    p.item_waves = bh * 8 <= waves ? 8 : bh * 4 <= 2 * int64_t(waves) ? 4 : 2;
+    const int64_t resident = int64_t(slots) * waves;
+    p.item_waves = bh * 8 <= resident ? 8 : bh * 4 <= 2 * resident ? 4 : 2;
+    p.item_waves = std::min(p.item_waves, waves);
     while (p.item_waves > 1 && (p.item_waves - 1) * 8 >= cap) p.item_waves /= 2;
     // A wave resolves the page of each of its steps into one lane: 64 steps of 8 tokens.
     const int64_t most = std::min<int64_t>(512 * p.item_waves, 2048);
     const int64_t want = (cap * bh / slots + 63) / 64 * 64;
     p.split_keys = int(std::min<int64_t>(most, std::max<int64_t>(want, 512)));
     p.splits = int(ceil_div(cap, p.split_keys));
-    const int groups = kWaves / p.item_waves;
-    p.more_blocks = int(std::min<int64_t>(slots, (bh * (p.splits - 1) + groups - 1) / groups));
+    const int groups = waves / p.item_waves;
+    p.more_blocks = int(std::min<int64_t>(slots, ceil_div(bh * (p.splits - 1), groups)));
     p.own_blocks = ceil_div(bh, groups);
     p.own_qt = 1;
   } else {
-    p.own_qt = max_tokens <= 32 ? 1 : max_tokens <= 64 ? 2 : 4;
+    p.own_qt = std::min(waves, max_tokens <= 32 ? 1 : max_tokens <= 64 ? 2 : 4);
     p.own_tiles = int(ceil_div(max_tokens, 32 * p.own_qt));
     p.split_keys = 2048;
     p.splits = int(ceil_div(cap + 1, p.split_keys));
@@ -1093,10 +1111,11 @@ bool whole_chunks(int d, int dtype) { return d * (dtype == kF32 ? 4 : 2) % 16 ==
 
 template <int DT, int DP>
 void launch_fast(const SharedArgs& a, const Plan& p) {
-  const int blocks = int(p.more_blocks + p.prefix_items + p.own_blocks);
-  if (!a.k) shared_kernel<DT, DP, kRowsFull, false><<<blocks, kThreads>>>(a, p);
-  else if (a.g.dim == DP) shared_kernel<DT, DP, kRowsFull, true><<<blocks, kThreads>>>(a, p);
-  else shared_kernel<DT, DP, kRowsPadded, true><<<blocks, kThreads>>>(a, p);
+  constexpr int NT = Shape<DT, DP>::NT;
+  const int blocks = int(p.prefix_items + p.more_blocks + p.own_blocks);
+  if (!a.k) shared_kernel<DT, DP, kRowsFull, false><<<blocks, NT>>>(a, p);
+  else if (a.g.dim == DP) shared_kernel<DT, DP, kRowsFull, true><<<blocks, NT>>>(a, p);
+  else shared_kernel<DT, DP, kRowsPadded, true><<<blocks, NT>>>(a, p);
   const int64_t pairs = int64_t(a.rows) * a.g.heads;
   constexpr int LANES = DP / 4;
   if (p.pieces >= kManyPieces) shared_merge_kernel<DT, DP, kWave / LANES><<<int(ceil_div(pairs, kMergeThreads / kWave)), kMergeThreads>>>(a, p);
