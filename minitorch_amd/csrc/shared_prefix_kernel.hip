@@ -236,11 +236,15 @@ __device__ __forceinline__ const T* page_of(const SharedArgs& a, const uint64_t*
   return page_in_slab<T>(a.g.num_slabs <= kLdsSlabs ? s_slabs[slab] : a.slabs[slab], physical, a.g, head);
 }
 
-// How the launch is cut (made on the host).
+// How the launch is cut (made on the host). The prefix is units of prefix_unit keys;
+// a (head, tile of 32 qt queries) has tile_units of them, all heads' tiles in a
+// row, and a workgroup takes the next item_units: the same work for each, a piece
+// of a tile or the end of one and the start of the next.
 struct Plan {
-  // prefix: tiles of 32 qt queries, pieces of piece_keys keys (a multiple of 32)
-  int qt, tiles, pieces, piece_keys;
-  int64_t prefix_items;
+  int waves;  // of a workgroup
+  int qt, tiles, prefix_unit, tile_units, item_units;
+  int pieces;  // most pieces a tile is cut into
+  int64_t units, prefix_items;
   // own keys: splits of split_keys
   int split_keys, splits;
   // decode: waves per item and workgroups that take the rows of several splits
@@ -250,6 +254,14 @@ struct Plan {
   int64_t own_blocks;
   float* partials;
 };
+
+// The first item that works on a tile (tile: head * tiles + tile), and how many do.
+__device__ __forceinline__ int first_item(const Plan& p, int tile) {
+  return int(unsigned(tile) * unsigned(p.tile_units) / unsigned(p.item_units));
+}
+__device__ __forceinline__ int pieces_of(const Plan& p, int tile) {
+  return p.units ? int((unsigned(tile + 1) * unsigned(p.tile_units) - 1) / unsigned(p.item_units)) - first_item(p, tile) + 1 : 0;
+}
 
 // Elements of a query's partial: accumulators, maximum and denominator, 16-byte aligned.
 template <int DP>
@@ -262,20 +274,23 @@ __device__ __forceinline__ float* part_of(const SharedArgs& a, const Plan& p, in
 
 // Waves of a workgroup: four where their operands take 256 registers a lane, so
 // that two workgroups still share a compute unit -- a prefix item and own ones
-// (rows of 512 bytes stay with eight, for the sake of their rounds).
-constexpr int shape_waves(int row_bytes) { return row_bytes == 256 ? 4 : 8; }
+// (rows of 512 bytes stay with eight, for the sake of their rounds). Many rows of
+// several queries take eight all the same: tiles of 128 queries of head dim 128 ask the
+// caches for 32 KB every 4 MFLOP, more than they give (24 prompts behind 8100 tokens x
+// 16 heads: MEASURE_WIDE).
+constexpr int shape_waves(int row_bytes, bool wide) { return row_bytes == 256 && !wide ? 4 : 8; }
 
 // Staged keys of a workgroup: two halves of kHalf keys, K and V each. A wave takes
 // blocks of 32 keys: with few waves per query group (KG <= kHalf / 32) a round is
 // one half, staged while the other is computed; with more, both halves at once.
-template <int DT, int DP>
+template <int DT, int DP, int WAVES>
 struct Shape {
   static constexpr int ES = elem_bytes<DT>();
   static constexpr int EC = 16 / ES;          // elements per 16-byte chunk
   static constexpr int CPR = DP / EC;         // chunks per row
   static constexpr int RW = kWave / CPR;      // rows one load instruction of a wave fills
   static constexpr int kRowBytes = DP * ES;
-  static constexpr int W = shape_waves(kRowBytes);
+  static constexpr int W = WAVES;
   static constexpr int NT = W * kWave;
   static constexpr int kHalf = kRowBytes == 128 ? 128 : 64;
   static constexpr int kBlocks = kHalf / 32;
@@ -336,17 +351,19 @@ struct Tile {
 // kernels'; fp16's are taken 2^kHalfShift larger, whose low parts would
 // otherwise end at 2^-24. The exponentials' reference moves when a score exceeds
 // it by kRescale only.
-template <int DT, int DP>
+template <int DT, int DP, int W>
 __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, int head, char* s_raw,
                                             typename Elem<DT>::T const** s_page, uint64_t* s_slabs, int* s_missing) {
   using T = typename Elem<DT>::T;
-  using S = Shape<DT, DP>;
-  constexpr int EC = S::EC, CPR = S::CPR, NC = S::NC, DT32 = S::DT32, QW = S::QW, W = S::W, NT = S::NT;
+  using S = Shape<DT, DP, W>;
+  constexpr int EC = S::EC, CPR = S::CPR, NC = S::NC, DT32 = S::DT32, QW = S::QW, NT = S::NT;
   constexpr float kShift = DT == kF16 ? kHalfShift : 0.f;
   constexpr int CH = DP == 64 ? 4 : 2;  // chains of an fp32 block's sums
   const Geometry& g = a.g;
   const int dim = g.dim, chunks = dim / EC;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // keeps this tile's terms out of the registers of the tiles before
+  const int lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qt_n = t.qt, kg_n = W / qt_n;
   const int kg = wave / qt_n, qt = wave - kg * qt_n;
@@ -440,52 +457,9 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
   const int64_t own_limit = t.limit + qi;
   const int last_key = int(own_limit < t.k1 ? own_limit : t.k1 - 1);  // of this lane's query
 
-  // One block of 32 keys from `base` on, at row `at` of half h.
-  auto block = [&](int base, int h, int at) {
-    const T* const s_k = reinterpret_cast<const T*>(s_raw + h * 2 * S::kPlane) + at * DP;
-    const T* const s_v = s_k + S::kPlane / S::ES;
-    // lane holds keys base + 8 (i / 4) + 4 grp + i % 4 of query qi
-    floatx16 sc;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
-    auto read_k = [&](int s) {
-      const int p = DT == kF32 ? CPR / 2 * grp + s : 2 * s + grp;
-      return *reinterpret_cast<const u32x4*>(s_k + col * DP + S::kpos(col, p) * EC);
-    };
-    if constexpr (DT == kF32) {
-      // short chains of sums
-      floatx16 part[CH];
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[j][i] = 0.f;
-#pragma unroll
-      for (int s = 0; s < QW; ++s) {
-        const u32x4 kf = read_k(s);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          floatx16& c = part[j % CH];
-          c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[j]), __uint_as_float(qv[s][j]), c, 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = (part[0][i] + part[1][i]) + (CH == 4 ? part[CH - 2][i] + part[CH - 1][i] : 0.f);
-    } else {
-#pragma unroll
-      for (int s = 0; s < QW; ++s) sc = mfma32<DT>(read_k(s), qv[s], sc);
-    }
-    // limits, only for blocks that reach past one (a wave-uniform test)
-    if (base + 31 > t.limit + q0 || base + 32 > t.k1) {
-      const int last = last_key - base - 4 * grp;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = 8 * (i >> 2) + (i & 3) > last ? -INFINITY : sc[i];
-        asm volatile("" : "+v"(x));  // keeps this a branch: 46 instructions of a block's 190 without it
-        sc[i] = x;
-      }
-    }
-    // (each lane asks for its own half of the keys; a query's first ones, m = -inf, too)
-    const float mine = largest(sc);
+  // A score past the reference by kRescale moves it. (Each lane asks for its own
+  // half of the keys; a query's first ones, m = -inf, move it too.)
+  auto refer = [&](float mine) {
     if (__any(mine > threshold)) {
       const float mn = fmaxf(m, max_halves(mine) * a.qscale);
       const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
@@ -497,7 +471,10 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
       m = mn;
       threshold = (m + kRescale) * unscale;
     }
-    const float ref = m == -INFINITY ? 0.f : m - kShift;
+    return m == -INFINITY ? 0.f : m - kShift;
+  };
+  // The scores' weights, added to the denominator.
+  auto weigh = [&](floatx16& sc, float ref) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = fast_exp2(fmaf(sc[i], a.qscale, -ref));
     float sum[8];
@@ -508,6 +485,85 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
 #pragma unroll
       for (int i = 0; i < w; ++i) sum[i] += sum[i + w];
     l += sum[0];
+  };
+  // K's operand s of the block of 32 keys at s_k, for S^T.
+  auto read_k = [&](const T* s_k, int s) {
+    const int p = DT == kF32 ? CPR / 2 * grp + s : 2 * s + grp;
+    return *reinterpret_cast<const u32x4*>(s_k + col * DP + S::kpos(col, p) * EC);
+  };
+  // O^T += V^T P^T for 16-bit types, 16 keys a step: slot j < 4 of a lane holds key
+  // 16 s + 4 grp + j, slot j >= 4 key 16 s + 8 + 4 grp + j - 4, in P as in V^T.
+  auto accumulate = [&](const T* s_v, const floatx16& sc) {
+    const int t16 = lane & 15;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t h2, l2;
+        SplitP<DT == kF32 ? kF16 : DT>::split(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
+        hi[w] = h2;
+        lo[w] = l2;
+      }
+      u32x4 vt[DT32];
+#pragma unroll
+      for (int d = 0; d < DT32; ++d) {
+        const int rr = 4 * grp + (t16 >> 2);
+        const int p = 4 * d + ((lane >> 4) & 1) * 2 + ((t16 & 3) >> 1);
+        const T* v_at = s_v + (16 * s + rr) * DP + S::vpos(rr, p) * 8 + (t16 & 1) * 4;
+        const uint2 x = read_transposed(v_at), y = read_transposed(v_at + 8 * DP);
+        vt[d] = u32x4{x.x, x.y, y.x, y.y};
+      }
+      // (no product waits for the one before it)
+#pragma unroll
+      for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], hi, o[d]);
+#pragma unroll
+      for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], lo, o[d]);
+    }
+  };
+  auto keys_at = [&](int h, int at) { return reinterpret_cast<const T*>(s_raw + h * 2 * S::kPlane) + at * DP; };
+
+  // One block of 32 keys from `base` on, at row `at` of half h: lane holds the scores of
+  // keys base + 8 (i / 4) + 4 grp + i % 4 of query qi.
+  auto block = [&](int base, int h, int at) {
+    const T* const s_k = keys_at(h, at);
+    const T* const s_v = s_k + S::kPlane / S::ES;
+    floatx16 sc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+    if constexpr (DT == kF32) {
+      // short chains of sums
+      floatx16 part[CH];
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[j][i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < QW; ++s) {
+        const u32x4 kf = read_k(s_k, s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          floatx16& c = part[j % CH];
+          c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[j]), __uint_as_float(qv[s][j]), c, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = (part[0][i] + part[1][i]) + (CH == 4 ? part[CH - 2][i] + part[CH - 1][i] : 0.f);
+    } else {
+#pragma unroll
+      for (int s = 0; s < QW; ++s) sc = mfma32<DT>(read_k(s_k, s), qv[s], sc);
+    }
+    // limits, only for blocks that reach past one (a wave-uniform test)
+    if (base + 31 > t.limit + q0 || base + 32 > t.k1) {
+      const int last = last_key - base - 4 * grp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = 8 * (i >> 2) + (i & 3) > last ? -INFINITY : sc[i];
+        asm volatile("" : "+v"(x));  // keeps this a branch: 46 instructions of a block's 190 without it
+        sc[i] = x;
+      }
+    }
+    weigh(sc, refer(largest(sc)));
     if constexpr (DT == kF32) {
       // a block's sums start at zero, in chains, and are added to the running ones
 #pragma unroll
@@ -528,35 +584,27 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
           o[d][i] += (ob[0][i] + ob[1][i]) + (CH == 4 ? ob[CH - 2][i] + ob[CH - 1][i] : 0.f);
       }
     } else {
-      // 16 keys a step: slot j < 4 of a lane holds key 16 s + 4 grp + j, slot j
-      // >= 4 key 16 s + 8 + 4 grp + j - 4, in P as in V^T
-      const int t16 = lane & 15;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4 hi, lo;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t h2, l2;
-          SplitP<DT>::split(sc[8 * s + 2 * w], sc[8 * s + 2 * w + 1], h2, l2);
-          hi[w] = h2;
-          lo[w] = l2;
-        }
-        u32x4 vt[DT32];
-#pragma unroll
-        for (int d = 0; d < DT32; ++d) {
-          const int rr = 4 * grp + (t16 >> 2);
-          const int p = 4 * d + ((lane >> 4) & 1) * 2 + ((t16 & 3) >> 1);
-          const T* v_at = s_v + (16 * s + rr) * DP + S::vpos(rr, p) * 8 + (t16 & 1) * 4;
-          const uint2 x = read_transposed(v_at), y = read_transposed(v_at + 8 * DP);
-          vt[d] = u32x4{x.x, x.y, y.x, y.y};
-        }
-        // (no product waits for the one before it)
-#pragma unroll
-        for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], hi, o[d]);
-#pragma unroll
-        for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], lo, o[d]);
-      }
+      accumulate(s_v, sc);
     }
+  };
+  // Two blocks, both whole and within the limits, at rows at0 and at1 (16-bit types,
+  // where a lane has registers for it): their products take turns, and the reference is
+  // looked at once.
+  auto two_blocks = [&](int h, int at0, int at1) {
+    const T *const k0 = keys_at(h, at0), *const k1 = keys_at(h, at1);
+    floatx16 s0, s1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s0[i] = s1[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < QW; ++s) {
+      s0 = mfma32<DT>(read_k(k0, s), qv[s], s0);
+      s1 = mfma32<DT>(read_k(k1, s), qv[s], s1);
+    }
+    const float ref = refer(fmaxf(largest(s0), largest(s1)));
+    weigh(s0, ref);
+    weigh(s1, ref);
+    accumulate(k0 + S::kPlane / S::ES, s0);
+    accumulate(k1 + S::kPlane / S::ES, s1);
   };
 
   const bool both = kg_n > S::kBlocks;  // rounds of both halves
@@ -584,12 +632,21 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
       wait_staged<0>();
       __syncthreads();  // the half's keys are there, and the half before is done with
       if (k + S::kHalf < t.k1) stage(k + S::kHalf, h ^ 1);
-      if (live)
-        for (int at = kg * 32; at < S::kHalf; at += kg_n * 32) {
+      if (live) {
+        const int step = kg_n * 32;
+        int at = kg * 32;
+        if constexpr (DT != kF32 && S::SW == 2)
+          for (; at + step < S::kHalf; at += 2 * step) {
+            const int past = k + at + step + 32;
+            if (past > t.k1 || past - 1 > t.limit + q0) break;
+            two_blocks(h, at, at + step);
+          }
+        for (; at < S::kHalf; at += step) {
           const int base = k + at;
           if (base >= t.k1 || base > t.limit + min(q0 + 31, t.nq - 1)) break;
           block(base, h, at);
         }
+      }
     }
   }
 
@@ -650,7 +707,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
 // All threads of the workgroup enter (barriers); `on` where the group has an item.
 // What does not depend on the row's length -- table entries, query, new token --
 // is loaded with it, in one round trip.
-template <int DT, int DP, Rows FULL>
+template <int DT, int DP, int WAVES, Rows FULL>
 __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, bool on, int row, int head, int split,
                                             float* s_state, uint64_t* s_slabs, bool& slabs_there) {
   using T = typename Elem<DT>::T;
@@ -660,7 +717,6 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
   const Geometry& g = a.g;
   const int dim = FULL == kRowsFull ? DP : g.dim;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & (kWave - 1);
-  constexpr int WAVES = Shape<DT, DP>::W;
   const int W = p.item_waves, gw = wave % W, first_wave = wave - gw;
   const int col0 = C::first_col(lane % G), tok = lane / G;
   // before the prefix items' waves, whose products leave these few turns to ask for more keys
@@ -812,10 +868,10 @@ __device__ __forceinline__ void stream_item(const SharedArgs& a, const Plan& p, 
 // The rows of several splits: every workgroup counts them (rows in chunks of a thread
 // each) and takes its share. They start before the other rows, which are short
 // then, so that none is left alone at the end.
-template <int DT, int DP, Rows FULL>
+template <int DT, int DP, int WAVES, Rows FULL>
 __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, int block, float* s_state, uint64_t* s_slabs,
                                             int* s_count) {
-  constexpr int WAVES = Shape<DT, DP>::W, NT = WAVES * kWave;
+  constexpr int NT = WAVES * kWave;
   const Geometry& g = a.g;
   const int tid = threadIdx.x, groups = WAVES / p.item_waves, group = (tid >> 6) / p.item_waves;
   const int64_t cap = int64_t(g.columns) * g.page_size;
@@ -846,47 +902,58 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
       for (int step = NT / 2; step > 0; step >>= 1)
         if (s_count[i + step - 1] <= x) i += step;
       const int before = i ? s_count[i - 1] : 0;
-      stream_item<DT, DP, FULL>(a, p, on, on ? r0 + i : 0, head, x - before, s_state, s_slabs, slabs_there);
+      stream_item<DT, DP, WAVES, FULL>(a, p, on, on ? r0 + i : 0, head, x - before, s_state, s_slabs, slabs_there);
     }
     set -= sets;
   }
 }
 
-template <int DT, int DP, Rows FULL, bool DECODE>
-__global__ __launch_bounds__((Shape<DT, DP>::NT)) __attribute__((amdgpu_waves_per_eu((Shape<DT, DP>::SW))))
+template <int DT, int DP, int W, Rows FULL, bool DECODE>
+__global__ __launch_bounds__((Shape<DT, DP, W>::NT)) __attribute__((amdgpu_waves_per_eu((Shape<DT, DP, W>::SW))))
 void shared_kernel(SharedArgs a, Plan p) {
   using T = typename Elem<DT>::T;
-  using S = Shape<DT, DP>;
+  using S = Shape<DT, DP, W>;
   __shared__ const T* s_page[kPages];
   __shared__ uint64_t s_slabs[kLdsSlabs];
   __shared__ int s_missing;
   __shared__ __align__(16) char s_raw[S::kLds];
   const Geometry& g = a.g;
-  // The prefix items first: they are the long ones, at most one a compute unit
-  // where own items follow, which then take the rest of it.
+  // The prefix items first: they are the long ones, one a compute unit where own
+  // items follow, which then take the rest of it. Neighbours go to one XCD (the
+  // workgroups of a launch are dealt to the eight in turn), so that the tiles of a
+  // head share its keys in that XCD's L2.
   int index = int(blockIdx.x);
   if (index < p.prefix_items) {
-    // (piece, head, tile), the tiles of a piece side by side
-    const int ph = index / p.tiles, tile = index - ph * p.tiles;
-    const int piece = ph / g.heads, head = ph - piece * g.heads;
-    const int64_t row = int64_t(tile) * 32 * p.qt;
-    Tile t;
-    t.q = static_cast<const T*>(a.q) + row * a.q_r + int64_t(head) * g.dim;
-    t.nq = int(min(int64_t(32 * p.qt), a.rows - row));
-    t.qt = p.qt;
-    t.table_row = a.prefix_table;
-    t.columns = a.prefix_columns;
-    t.k0 = piece * p.piece_keys;
-    t.k1 = min(a.prefix, t.k0 + p.piece_keys);
-    t.limit = INT_MAX;
-    t.part = part_of<DP>(a, p, piece, head, row);
-    attend_tile<DT, DP>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
+    const int whole = int(p.prefix_items) & ~7;
+    if (index < whole) index = (index & 7) * (whole >> 3) + (index >> 3);
+    const int end = int(min(p.units, int64_t(index + 1) * p.item_units));
+#pragma unroll 1
+    for (int at = index * p.item_units; at < end;) {
+      const int head_tile = __builtin_amdgcn_readfirstlane(int(unsigned(at) / unsigned(p.tile_units)));
+      const int unit = at - head_tile * p.tile_units, n = min(p.tile_units - unit, end - at);
+      const int head = __builtin_amdgcn_readfirstlane(int(unsigned(head_tile) / unsigned(p.tiles)));
+      const int tile = head_tile - head * p.tiles;
+      const int64_t row = int64_t(tile) * 32 * p.qt;
+      Tile t;
+      t.q = static_cast<const T*>(a.q) + row * a.q_r + int64_t(head) * g.dim;
+      t.nq = int(min(int64_t(32 * p.qt), a.rows - row));
+      t.qt = p.qt;
+      t.table_row = a.prefix_table;
+      t.columns = a.prefix_columns;
+      t.k0 = unit * p.prefix_unit;
+      t.k1 = min(a.prefix, (unit + n) * p.prefix_unit);
+      t.limit = INT_MAX;
+      t.part = part_of<DP>(a, p, index - __builtin_amdgcn_readfirstlane(first_item(p, head_tile)), head, row);
+      attend_tile<DT, DP, W>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
+      at += n;
+      if (at < end) __syncthreads();  // the LDS is done with
+    }
     return;
   }
   index -= int(p.prefix_items);
   if constexpr (DECODE) {
     if (index < p.more_blocks) {
-      stream_more<DT, DP, FULL>(a, p, index, reinterpret_cast<float*>(s_raw), s_slabs, reinterpret_cast<int*>(s_page));
+      stream_more<DT, DP, W, FULL>(a, p, index, reinterpret_cast<float*>(s_raw), s_slabs, reinterpret_cast<int*>(s_page));
       return;
     }
     index -= p.more_blocks;
@@ -895,7 +962,7 @@ void shared_kernel(SharedArgs a, Plan p) {
     const bool on = item < int64_t(a.b) * g.heads;
     const int row = on ? int(item / g.heads) : 0;
     bool slabs_there = false;
-    stream_item<DT, DP, FULL>(a, p, on, row, on ? int(item - int64_t(row) * g.heads) : 0, -1,
+    stream_item<DT, DP, W, FULL>(a, p, on, row, on ? int(item - int64_t(row) * g.heads) : 0, -1,
                               reinterpret_cast<float*>(s_raw), s_slabs, slabs_there);
   } else {
     // (split, request, tile, head)
@@ -921,7 +988,7 @@ void shared_kernel(SharedArgs a, Plan p) {
     t.k1 = int(min(end, k0 + p.split_keys));
     t.limit = int64_t(rq.length) + q0;
     t.part = part_of<DP>(a, p, p.pieces + split, head, row);
-    attend_tile<DT, DP>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
+    attend_tile<DT, DP, W>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
   }
 }
 
@@ -970,7 +1037,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedArgs 
       all.add(*reinterpret_cast<const float2*>(x + DP), *reinterpret_cast<const float4*>(x + dd));
     }
   };
-  if (row < a.rows) join(0, p.pieces);
+  if (row < a.rows) join(0, pieces_of(p, head * p.tiles + int(row) / (32 * p.qt)));
   int r = int(row);
   if (a.cu_tokens) {
     // the request of the workgroup's first row: as many as start at or before it,
@@ -1060,10 +1127,13 @@ int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 // How a launch is cut.
 Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int columns, int max_tokens, int dtype, bool decode) {
   const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
-  const int row_bytes = (d <= 64 ? 64 : 128) * (dtype == kF32 ? 4 : 2), waves = shape_waves(row_bytes);
-  const int slots = (row_bytes == 512 ? 1 : 2) * cus;  // workgroups that are resident at once
+  const int row_bytes = (d <= 64 ? 64 : 128) * (dtype == kF32 ? 4 : 2);
+  const bool wide = !decode && dtype != kF32 && rows > 128;
+  const int waves = shape_waves(row_bytes, wide);
+  const int slots = (row_bytes * waves <= 1024 ? 2 : 1) * cus;  // workgroups that are resident at once
   const int64_t cap = int64_t(columns) * page_size, bh = int64_t(b) * h;
   Plan p{};
+  p.waves = waves;
   // Prefix tiles: the queries' groups of 32 over tiles of 1, 2, 4 or 8 groups,
   // where a tile costs its groups and about one more.
   int64_t best = INT64_MAX;
@@ -1073,31 +1143,57 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
   }
   p.tiles = int(ceil_div(rows, 32 * p.qt));
   if (prefix > 0) {
-    const int64_t items = int64_t(p.tiles) * h;
-    const int64_t want = std::max<int64_t>(1, cus / items);
-    const int least = items * ceil_div(prefix, 256) < cus / 4 ? 64 : 256;  // keys of a piece
-    int64_t pieces = std::min<int64_t>(want, ceil_div(prefix, least));
-    pieces = std::max<int64_t>(pieces, ceil_div(prefix, kPages * page_size));
-    p.piece_keys = int(ceil_div(ceil_div(prefix, pieces), 32) * 32);
-    p.pieces = int(ceil_div(prefix, p.piece_keys));
-    p.prefix_items = items * p.pieces;
+    // Units of a staged half. One item a compute unit, which leaves half of its
+    // places (a quarter of the compute units, where an item takes a whole one) to
+    // the own items; tiles of few queries wait for memory more than they compute
+    // and fill every place. us, items of half as many, as many and twice as many
+    // compute units: 256 decode rows x 16 heads behind 16001 tokens 88, 76 and 94; 64
+    // requests of 1-20 tokens x 12 behind 4096 50, 42 and 49; one decode row x 12
+    // behind 32000 40, 29 and 27; 24 prompts x 16 heads of 128 behind 8100 (eight waves)
+    // 358, 378 and 390, with three quarters 356.
+    // Pieces of 256 keys at least unless few would be left (4 rows fp32 x 12 heads behind
+    // 200: 10.5 in pieces of 64, 13 whole), cut at the tiles' ends where that keeps nine
+    // tenths of the items busy, for the fewest pieces.
+    const int64_t head_tiles = int64_t(p.tiles) * h;
+    const int64_t want = 2 * p.qt < waves ? slots : slots > cus || dtype == kF32 ? cus : 3 * int64_t(cus) / 4;
+    p.prefix_unit = row_bytes == 128 ? 128 : 64;
+    int64_t units = ceil_div(prefix, p.prefix_unit);
+    if (head_tiles * ceil_div(prefix, 256) < cus / 4) {
+      p.prefix_unit = 64;
+      units = ceil_div(prefix, 64);
+      p.item_units = 1;
+    } else {
+      p.item_units = int(std::max<int64_t>(256 / p.prefix_unit, ceil_div(head_tiles * units, want)));
+    }
+    p.item_units = int(std::min<int64_t>(p.item_units, int64_t(kPages) * page_size / p.prefix_unit));
+    const int64_t even = ceil_div(units, ceil_div(units, p.item_units));  // units of pieces of one length
+    const int64_t items = head_tiles * ceil_div(units, even), rounds = ceil_div(items, want);
+    if (10 * items >= 9 * rounds * want || even == units) {
+      p.item_units = int(even);
+      units = ceil_div(units, even) * even;
+    }
+    p.tile_units = int(units);
+    p.units = head_tiles * units;
+    p.prefix_items = ceil_div(p.units, p.item_units);
+    p.pieces = int(units % p.item_units == 0   ? units / p.item_units
+                   : p.item_units % units == 0 ? 1
+                                               : (units - 2) / p.item_units + 2);
   }
   if (decode) {
     const int64_t resident = int64_t(slots) * waves;
     p.item_waves = bh * 8 <= resident ? 8 : bh * 4 <= 2 * resident ? 4 : 2;
     p.item_waves = std::min(p.item_waves, waves);
     while (p.item_waves > 1 && (p.item_waves - 1) * 8 >= cap) p.item_waves /= 2;
-    // A wave resolves the page of each of its steps into one lane: 64 steps of 8 tokens.
-    const int64_t most = std::min<int64_t>(512 * p.item_waves, 2048);
-    const int64_t want = (cap * bh / slots + 63) / 64 * 64;
-    p.split_keys = int(std::min<int64_t>(most, std::max<int64_t>(want, 512)));
+    // Splits of 512 tokens: a wave resolves the page of each of its steps into one
+    // lane, 64 steps of 8 tokens. Longer ones for tables of more than 64.
+    p.split_keys = int(std::min<int64_t>(512 * p.item_waves, std::max<int64_t>(512, ceil_div(cap, 64 * 64) * 64)));
     p.splits = int(ceil_div(cap, p.split_keys));
     const int groups = waves / p.item_waves;
     p.more_blocks = p.splits > 1 ? int(std::min<int64_t>(slots, ceil_div(bh * p.splits, groups))) : 0;
     p.own_blocks = ceil_div(bh, groups);
     p.own_qt = 1;
   } else {
-    p.own_qt = std::min(waves, max_tokens <= 32 ? 1 : max_tokens <= 64 ? 2 : 4);
+    p.own_qt = std::min(waves, max_tokens <= 32 ? 1 : max_tokens <= 64 ? 2 : max_tokens <= 128 ? 4 : 8);
     p.own_tiles = int(ceil_div(max_tokens, 32 * p.own_qt));
     p.split_keys = 2048;
     p.splits = int(ceil_div(cap + 1, p.split_keys));
@@ -1107,7 +1203,7 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
 }
 
 // Whether one launch can hold the plan's workgroups.
-bool plan_fits(const Plan& p) { return p.prefix_items + p.own_blocks < (int64_t(1) << 30); }
+bool plan_fits(const Plan& p) { return p.units < (int64_t(1) << 31) - p.item_units && p.prefix_items + p.own_blocks < (int64_t(1) << 30); }
 
 size_t plan_bytes(const Plan& p, int rows, int h, int d) {
   return size_t(p.pieces + p.splits) * h * rows * (d <= 64 ? part_row<64>() : part_row<128>()) * sizeof(float);
@@ -1116,13 +1212,23 @@ size_t plan_bytes(const Plan& p, int rows, int h, int d) {
 // Rows that the fast path takes: whole 16-byte chunks.
 bool whole_chunks(int d, int dtype) { return d * (dtype == kF32 ? 4 : 2) % 16 == 0; }
 
+template <int DT, int DP, int W>
+void launch_waves(const SharedArgs& a, const Plan& p) {
+  const int blocks = int(p.prefix_items + p.more_blocks + p.own_blocks);
+  if (!a.k) shared_kernel<DT, DP, W, kRowsFull, false><<<blocks, W * kWave>>>(a, p);
+  else if (a.g.dim == DP) shared_kernel<DT, DP, W, kRowsFull, true><<<blocks, W * kWave>>>(a, p);
+  else shared_kernel<DT, DP, W, kRowsPadded, true><<<blocks, W * kWave>>>(a, p);
+}
+
 template <int DT, int DP>
 void launch_fast(const SharedArgs& a, const Plan& p) {
-  constexpr int NT = Shape<DT, DP>::NT;
-  const int blocks = int(p.prefix_items + p.more_blocks + p.own_blocks);
-  if (!a.k) shared_kernel<DT, DP, kRowsFull, false><<<blocks, NT>>>(a, p);
-  else if (a.g.dim == DP) shared_kernel<DT, DP, kRowsFull, true><<<blocks, NT>>>(a, p);
-  else shared_kernel<DT, DP, kRowsPadded, true><<<blocks, NT>>>(a, p);
+  constexpr int row_bytes = DP * elem_bytes<DT>();
+  if constexpr (shape_waves(row_bytes, false) == 4) {
+    if (p.waves == 4) launch_waves<DT, DP, 4>(a, p);
+    else shared_kernel<DT, DP, 8, kRowsFull, false><<<int(p.prefix_items + p.own_blocks), 8 * kWave>>>(a, p);
+  } else {
+    launch_waves<DT, DP, 8>(a, p);
+  }
   const int64_t pairs = int64_t(a.rows) * a.g.heads;
   constexpr int LANES = DP / 4;
   if (p.pieces >= kManyPieces) shared_merge_kernel<DT, DP, kWave / LANES><<<int(ceil_div(pairs, kMergeThreads / kWave)), kMergeThreads>>>(a, p);
