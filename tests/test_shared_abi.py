@@ -32,7 +32,8 @@ TABLES = dict(table=16, slots=16, positions=16, cu=16, lengths=16, tokens=16, pa
 
 @pytest.mark.parametrize('bad', [
     dict(table=None), dict(slots=None), dict(positions=None), dict(cu=None), dict(lengths=None), dict(pages=None),
-    dict(b=0), dict(b=65536), dict(rows=0), dict(page_count=-1), dict(columns=0), dict(columns=2 ** 29 + 1),
+    dict(b=0), dict(b=65536), dict(rows=0), dict(rows=2 ** 24), dict(page_count=-1),
+    dict(page_count=2 ** 30 + 1), dict(columns=0), dict(columns=2 ** 29 + 1),
     dict(page_size=12), dict(page_size=64), dict(prefix=-1), dict(b=65535, columns=32769),
     dict(b=1, columns=2 ** 27, page_size=16)])
 def test_batch_tables_refuses(bad):
