@@ -15,7 +15,11 @@
  * Workspace: partial results, of the size that mt_paged_shared_workspace_bytes
  * reports for the same sizes (0: none is needed, and it may be null), 16-byte
  * aligned, with no content to keep between calls; calls that share one must not
- * overlap, nor must replays of graphs captured with it.
+ * overlap, nor must replays of graphs captured with it. `out` overlaps no input.
+ * Sizes: h <= 65535 / b; rows * h * d, prefix and own tokens of a table together
+ * below 2^31; for rows of whole 16-byte chunks also rows * h < 2^26, and at most 2^22
+ * pieces of work of one kind (tiles of up to 256 rows x the cuts of the longest
+ * keys). What is past them is refused with hipErrorInvalidValue.
  */
 #ifndef MT_SHARED_H
 #define MT_SHARED_H

@@ -249,8 +249,9 @@ struct Plan {
   int split_keys, splits;
   // decode: waves per item and workgroups that take the rows of several splits
   int item_waves, more_blocks;
-  // several queries: tiles of 32 own_qt queries
+  // several queries: tiles of 32 own_qt queries; `listed` workgroups look up their items
   int own_qt, own_tiles;
+  bool listed;
   int64_t own_blocks;
   float* partials;
 };
@@ -277,7 +278,7 @@ __device__ __forceinline__ float* part_of(const SharedArgs& a, const Plan& p, in
 // (rows of 512 bytes stay with eight, for the sake of their rounds). Many rows of
 // several queries take eight all the same: tiles of 128 queries of head dim 128 ask the
 // caches for 32 KB every 4 MFLOP, more than they give (24 prompts behind 8100 tokens x
-// 16 heads: MEASURE_WIDE).
+// 16 heads: 354 us with eight, 387 with four).
 constexpr int shape_waves(int row_bytes, bool wide) { return row_bytes == 256 && !wide ? 4 : 8; }
 
 // Staged keys of a workgroup: two halves of kHalf keys, K and V each. A wave takes
@@ -908,7 +909,94 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
   }
 }
 
-template <int DT, int DP, int W, Rows FULL, bool DECODE>
+// Own keys of several queries: an item is a tile of a request's queries, one of its
+// splits and a head. The host knows bounds only: each request as long as the longest,
+// each context as long as the table. Up to eight rounds of such workgroups those without
+// work cost little (2 us of 120 at 3000); where the bounds give more, eight rounds
+// count the items that there are (kListed requests at once) and share them out: 500
+// requests of one token and 12 prompts of 500-2048 behind 2048 tokens, 12 heads, table
+// of 8192: 366 us, with a workgroup for each of 245000 bounds 1230.
+constexpr int kListed = 256;
+
+template <int DT, int DP, int W>
+__device__ __forceinline__ void own_item(const SharedArgs& a, const Plan& p, int r, const Request& rq, int tile, int split,
+                                         int head, char* s_raw, typename Elem<DT>::T const** s_page, uint64_t* s_slabs,
+                                         int* s_missing) {
+  using T = typename Elem<DT>::T;
+  const Geometry& g = a.g;
+  const int q0 = tile * 32 * p.own_qt;
+  if (rq.length < 0 || q0 >= rq.tokens) return;
+  Tile t;
+  t.nq = min(32 * p.own_qt, rq.tokens - q0);
+  // a key past the table is a missing page: one of them is enough
+  const int64_t end = min(int64_t(rq.length) + q0 + t.nq, int64_t(g.columns) * g.page_size + 1);
+  const int64_t k0 = int64_t(split) * p.split_keys;
+  if (k0 >= end) return;
+  const int64_t row = int64_t(rq.row0) + q0;
+  t.q = static_cast<const T*>(a.q) + row * a.q_r + int64_t(head) * g.dim;
+  t.qt = p.own_qt;
+  while (t.qt > 1 && 16 * t.qt >= t.nq) t.qt /= 2;  // few queries leave more waves to their keys
+  t.table_row = a.table + int64_t(r) * g.columns;
+  t.columns = g.columns;
+  t.k0 = int(k0);
+  t.k1 = int(min(end, k0 + p.split_keys));
+  t.limit = int64_t(rq.length) + q0;
+  t.part = part_of<DP>(a, p, p.pieces + split, head, row);
+  attend_tile<DT, DP, W>(a, t, head, s_raw, s_page, s_slabs, s_missing);
+}
+
+template <int DT, int DP, int W>
+__device__ __forceinline__ void listed_items(const SharedArgs& a, const Plan& p, int block, char* s_raw,
+                                             typename Elem<DT>::T const** s_page, uint64_t* s_slabs, int* s_missing,
+                                             int* s_count) {
+  const Geometry& g = a.g;
+  const int tid = threadIdx.x, tq = 32 * p.own_qt;
+  const int64_t cap = int64_t(g.columns) * g.page_size;
+  int64_t next = block;  // this workgroup's next item, less those of the requests before
+#pragma unroll 1
+  for (int r0 = 0; r0 < a.b; r0 += kListed) {
+    // tiles times splits of the last of them (an early tile's later splits are none)
+    int items = 0;
+    if (tid < kListed && r0 + tid < a.b) {
+      const Request rq = request_of(a, r0 + tid);
+      if (rq.length >= 0 && rq.tokens > 0) {
+        const int64_t end = min(int64_t(rq.length) + rq.tokens, cap + 1);
+        items = (rq.tokens + tq - 1) / tq * int((end + p.split_keys - 1) / p.split_keys);
+      }
+    }
+    int sum = wave_inclusive_add(items);
+    __syncthreads();  // the requests before are done with
+    if (tid < kListed && (tid & 63) == 63) s_count[kListed + (tid >> 6)] = sum;
+    __syncthreads();
+    if (tid < kListed) {
+      for (int w = 0; w < (tid >> 6); ++w) sum += s_count[kListed + w];
+      s_count[tid] = sum;
+    }
+    __syncthreads();
+    const int64_t all = int64_t(s_count[kListed - 1]) * g.heads;
+#pragma unroll 1
+    for (; next < all; next += p.own_blocks) {
+      const int x = __builtin_amdgcn_readfirstlane(int(next / g.heads));
+      const int head = __builtin_amdgcn_readfirstlane(int(next - int64_t(x) * g.heads));
+      int i = 0;  // the first request whose sum passes x
+#pragma unroll
+      for (int step = kListed / 2; step > 0; step >>= 1)
+        if (s_count[i + step - 1] <= x) i += step;
+      i = __builtin_amdgcn_readfirstlane(i);
+      const int item = x - (i ? __builtin_amdgcn_readfirstlane(s_count[i - 1]) : 0);
+      const Request rq = request_of(a, r0 + i);
+      const int tiles = max(1, (rq.tokens + tq - 1) / tq), split = item / tiles;
+      own_item<DT, DP, W>(a, p, r0 + i, rq, item - split * tiles, split, head, s_raw, s_page, s_slabs, s_missing);
+      __syncthreads();  // the LDS is done with
+    }
+    next -= all;
+  }
+}
+
+// Own: one new token per request; several, a workgroup per item; several, shared out.
+enum Own { kOwnToken, kOwnTiles, kOwnListed };
+
+template <int DT, int DP, int W, Rows FULL, Own OWN>
 __global__ __launch_bounds__((Shape<DT, DP, W>::NT)) __attribute__((amdgpu_waves_per_eu((Shape<DT, DP, W>::SW))))
 void shared_kernel(SharedArgs a, Plan p) {
   using T = typename Elem<DT>::T;
@@ -951,7 +1039,7 @@ void shared_kernel(SharedArgs a, Plan p) {
     return;
   }
   index -= int(p.prefix_items);
-  if constexpr (DECODE) {
+  if constexpr (OWN == kOwnToken) {
     if (index < p.more_blocks) {
       stream_more<DT, DP, W, FULL>(a, p, index, reinterpret_cast<float*>(s_raw), s_slabs, reinterpret_cast<int*>(s_page));
       return;
@@ -964,31 +1052,15 @@ void shared_kernel(SharedArgs a, Plan p) {
     bool slabs_there = false;
     stream_item<DT, DP, W, FULL>(a, p, on, row, on ? int(item - int64_t(row) * g.heads) : 0, -1,
                               reinterpret_cast<float*>(s_raw), s_slabs, slabs_there);
-  } else {
+  } else if constexpr (OWN == kOwnTiles) {
     // (split, request, tile, head)
-    int i = index / g.heads;
-    const int head = index - i * g.heads;
+    const int i = index / g.heads, head = index - i * g.heads;
     const int rt = i / p.own_tiles, tile = i - rt * p.own_tiles;
     const int split = rt / a.b, r = rt - split * a.b;
-    const Request rq = request_of(a, r);
-    const int q0 = tile * 32 * p.own_qt;
-    if (rq.length < 0 || q0 >= rq.tokens) return;
-    Tile t;
-    t.nq = min(32 * p.own_qt, rq.tokens - q0);
-    // a key past the table is a missing page: one of them is enough
-    const int64_t end = min(int64_t(rq.length) + q0 + t.nq, int64_t(g.columns) * g.page_size + 1);
-    const int64_t k0 = int64_t(split) * p.split_keys;
-    if (k0 >= end) return;
-    const int64_t row = int64_t(rq.row0) + q0;
-    t.q = static_cast<const T*>(a.q) + row * a.q_r + int64_t(head) * g.dim;
-    t.qt = p.own_qt;
-    t.table_row = a.table + int64_t(r) * g.columns;
-    t.columns = g.columns;
-    t.k0 = int(k0);
-    t.k1 = int(min(end, k0 + p.split_keys));
-    t.limit = int64_t(rq.length) + q0;
-    t.part = part_of<DP>(a, p, p.pieces + split, head, row);
-    attend_tile<DT, DP, W>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
+    own_item<DT, DP, W>(a, p, r, request_of(a, r), tile, split, head, s_raw, s_page, s_slabs, &s_missing);
+  } else {
+    __shared__ int s_count[kListed + kListed / kWave];
+    listed_items<DT, DP, W>(a, p, index, s_raw, s_page, s_slabs, &s_missing, s_count);
   }
 }
 
@@ -1118,7 +1190,7 @@ bool shared_shape(int b, int rows, int max_tokens, int h, int d, int page_size, 
          int64_t(b) * h <= 65535 && int64_t(rows) * h * d <= INT32_MAX && (page_size == 8 || page_size == 16 || page_size == 32) &&
          pps > 0 && num_slabs > 0 && int64_t(pps) * num_slabs <= INT32_MAX && prefix >= 0 && columns > 0 &&
          int64_t(b) * columns <= INT32_MAX && int64_t(columns) * page_size <= INT32_MAX - 4096 &&
-         int64_t(prefix) <= INT32_MAX - 4096 - int64_t(columns) * page_size && layers > 0 && layer >= 0 && layer < layers &&
+         int64_t(prefix) <= INT32_MAX - 32768 - int64_t(columns) * page_size && layers > 0 && layer >= 0 && layer < layers &&
          dtype >= 0 && dtype <= 2;
 }
 
@@ -1198,12 +1270,19 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
     p.split_keys = 2048;
     p.splits = int(ceil_div(cap + 1, p.split_keys));
     p.own_blocks = bh * p.own_tiles * p.splits;
+    // (256 requests of 1-8 tokens, 15400 bounds: 213 us listed, 240 not; 64 of 5, 3840: 33 and 32)
+    p.listed = p.own_blocks > 8 * slots;
+    if (p.listed) p.own_blocks = 8 * slots;
   }
   return p;
 }
 
-// Whether one launch can hold the plan's workgroups.
-bool plan_fits(const Plan& p) { return p.units < (int64_t(1) << 31) - p.item_units && p.prefix_items + p.own_blocks < (int64_t(1) << 30); }
+// Whether the launches can hold the plan's workgroups (2^32 threads), and the counts of
+// items their 32 bits.
+bool plan_fits(const Plan& p, int rows, int h) {
+  return p.units < (int64_t(1) << 31) - p.item_units && p.prefix_items < 1 << 22 && int64_t(rows) * h < 1 << 26 &&
+         int64_t(p.own_tiles) * p.splits < 1 << 22;
+}
 
 size_t plan_bytes(const Plan& p, int rows, int h, int d) {
   return size_t(p.pieces + p.splits) * h * rows * (d <= 64 ? part_row<64>() : part_row<128>()) * sizeof(float);
@@ -1213,22 +1292,20 @@ size_t plan_bytes(const Plan& p, int rows, int h, int d) {
 bool whole_chunks(int d, int dtype) { return d * (dtype == kF32 ? 4 : 2) % 16 == 0; }
 
 template <int DT, int DP, int W>
-void launch_waves(const SharedArgs& a, const Plan& p) {
-  const int blocks = int(p.prefix_items + p.more_blocks + p.own_blocks);
-  if (!a.k) shared_kernel<DT, DP, W, kRowsFull, false><<<blocks, W * kWave>>>(a, p);
-  else if (a.g.dim == DP) shared_kernel<DT, DP, W, kRowsFull, true><<<blocks, W * kWave>>>(a, p);
-  else shared_kernel<DT, DP, W, kRowsPadded, true><<<blocks, W * kWave>>>(a, p);
+void launch_tiles(const SharedArgs& a, const Plan& p) {
+  const int blocks = int(p.prefix_items + p.own_blocks);
+  if (p.listed) shared_kernel<DT, DP, W, kRowsFull, kOwnListed><<<blocks, W * kWave>>>(a, p);
+  else shared_kernel<DT, DP, W, kRowsFull, kOwnTiles><<<blocks, W * kWave>>>(a, p);
 }
 
 template <int DT, int DP>
 void launch_fast(const SharedArgs& a, const Plan& p) {
-  constexpr int row_bytes = DP * elem_bytes<DT>();
-  if constexpr (shape_waves(row_bytes, false) == 4) {
-    if (p.waves == 4) launch_waves<DT, DP, 4>(a, p);
-    else shared_kernel<DT, DP, 8, kRowsFull, false><<<int(p.prefix_items + p.own_blocks), 8 * kWave>>>(a, p);
-  } else {
-    launch_waves<DT, DP, 8>(a, p);
-  }
+  constexpr int W = shape_waves(DP * elem_bytes<DT>(), false);
+  const int blocks = int(p.prefix_items + p.more_blocks + p.own_blocks);
+  if (a.k && a.g.dim == DP) shared_kernel<DT, DP, W, kRowsFull, kOwnToken><<<blocks, W * kWave>>>(a, p);
+  else if (a.k) shared_kernel<DT, DP, W, kRowsPadded, kOwnToken><<<blocks, W * kWave>>>(a, p);
+  else if (p.waves == W) launch_tiles<DT, DP, W>(a, p);
+  else if constexpr (W == 4 && DT != kF32) launch_tiles<DT, DP, 8>(a, p);
   const int64_t pairs = int64_t(a.rows) * a.g.heads;
   constexpr int LANES = DP / 4;
   if (p.pieces >= kManyPieces) shared_merge_kernel<DT, DP, kWave / LANES><<<int(ceil_div(pairs, kMergeThreads / kWave)), kMergeThreads>>>(a, p);
@@ -1292,12 +1369,10 @@ int mt_paged_shared_workspace_bytes(int rows, int b, int h, int d, int page_size
                                     int max_tokens, int dtype, size_t* bytes) {
   if (!bytes || !shared_shape(b, rows, max_tokens, h, d, page_size, 1, 1, prefix_tokens, columns, 0, 1, dtype))
     return hipErrorInvalidValue;
-  *bytes = 0;
-  if (!whole_chunks(d, dtype)) return hipSuccess;
   size_t need = 0;
-  for (int decode = 0; decode < (max_tokens == 1 && rows == b ? 2 : 1); ++decode) {
+  for (int decode = 0; whole_chunks(d, dtype) && decode < (max_tokens == 1 && rows == b ? 2 : 1); ++decode) {
     const Plan p = make_plan(rows, b, h, d, page_size, prefix_tokens, columns, max_tokens, dtype, decode);
-    if (!plan_fits(p)) return hipErrorInvalidValue;
+    if (!plan_fits(p, rows, h)) return hipErrorInvalidValue;
     need = std::max(need, plan_bytes(p, rows, h, d));
   }
   *bytes = need;

@@ -1,5 +1,7 @@
 """mt_sched_batch_tables against the requests taken one by one on the host:
 whole tables, slot maps, positions and offsets, bit for bit."""
+import ctypes as ct
+
 import numpy as np
 import pytest
 
@@ -139,3 +141,41 @@ def test_many_requests():
     live = lengths >= 0
     pages = rng.integers(0, 10 ** 6, int((-(-(lengths + tokens) // 16) - -(-lengths // 16))[live].sum()))
     check(table, lengths, tokens, pages, rows=int(tokens[live].sum()) + 1)
+
+
+def test_lengths_and_tokens_at_their_ends():
+    table = np.full((300, 4), 9, np.int32)
+    most = 2 ** 31 - 1
+    lengths = np.array([most, 10, most - 3, 0, 20] + [0] * 295)
+    check(table, lengths, [5, 2, most, most, 3] + [most] * 295, np.arange(9), rows=700)
+    check(table, [most] * 300, [most] * 300, np.arange(9), rows=2 ** 13, page=32)
+
+
+def test_captured_call_replays():
+    lib = runtime().lib
+    lib.mt_graph_end.argtypes = [ct.POINTER(ct.c_void_p)]
+    lib.mt_graph_launch.argtypes = lib.mt_graph_destroy.argtypes = [ct.c_void_p]
+    b, rows, page, columns = 300, 2000, 16, 16
+    table, slots, positions = RawDeviceBuffer(4 * b * columns), RawDeviceBuffer(8 * rows), RawDeviceBuffer(4 * rows)
+    cu, lengths, tokens, pages = (RawDeviceBuffer(4 * n) for n in (b + 1, b, b, 900))
+    graph = ct.c_void_p()
+    for step in range(4):
+        t, L, n, p = random_step(50 + step, b, page, new=5 + step)
+        t = np.concatenate([t, np.full((b, columns - t.shape[1]), 77, np.int32)], 1)
+        p = np.concatenate([p, np.full(900 - len(p), 5, p.dtype)]).astype(np.int32)
+        for buffer, x in ((table, t), (lengths, L), (tokens, n), (pages, p), (positions, np.full(rows, np.float32(-7)))):
+            buffer.upload(x.astype(np.int32) if x.dtype == np.int64 else x)
+        if not graph:
+            assert lib.mt_graph_begin() == 0
+            paged_ops.batch_tables(table.ptr, slots.ptr, positions.ptr, cu.ptr, lengths.ptr, tokens.ptr, pages.ptr, b=b,
+                                   rows=rows, page_count=900, columns=columns, page_size=page, prefix_tokens=3)
+            assert lib.mt_graph_end(ct.byref(graph)) == 0
+        for _ in range(2):
+            assert lib.mt_graph_launch(graph) == 0
+        runtime().synchronize()
+        ref = plain(t, L, n, p, rows=rows, page=page, prefix=3)
+        got = (table.download(np.int32, t.size).reshape(t.shape), slots.download(np.int64, rows),
+               positions.download(np.float32, rows), cu.download(np.int32, b + 1))
+        for x, y in zip(got, ref):
+            assert np.array_equal(x, y)
+    assert lib.mt_graph_destroy(graph) == 0

@@ -105,10 +105,28 @@ def test_attentions_refuse_a_workspace_that_does_not_do(bad):
     assert _call(lib, 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], ATTEND, bad) == 1
 
 
-def test_attention_refuses_more_workgroups_than_a_launch_has():
-    # 65535 requests that might each bring 2^20 tokens
-    big = dict(b=65535, rows=2 ** 24, max_tokens=2 ** 20, h=1, d=64, columns=2 ** 15)
-    assert _call('shared_prefix_kernel', 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], ATTEND, big) == 1
+# Sizes that a launch's workgroups or the counts of its items do not hold, and ones
+# just below them.
+PLANS = [(dict(rows=2 ** 22, h=16, d=8), dict(rows=2 ** 22 - 1, h=16, d=8)),
+         (dict(rows=2 ** 22, max_tokens=2 ** 22, h=1, b=1, columns=2 ** 15, prefix=0),
+          dict(rows=2 ** 22, max_tokens=2 ** 22, h=1, b=1, columns=2 ** 15 - 200, prefix=0)),
+         (dict(rows=2 ** 22, h=1, b=1, prefix=2 ** 21), dict(rows=2 ** 22, h=1, b=1, prefix=2 ** 20))]
+
+
+@pytest.mark.parametrize('bad,good', PLANS)
+def test_workspace_refuses_more_than_a_launch_has(bad, good):
+    types, size = [I] * 9 + [ct.POINTER(ct.c_size_t)], ct.c_size_t(7)
+    args = dict(SIZE, size=ct.byref(size))
+    assert _call('shared_prefix_kernel', 'mt_paged_shared_workspace_bytes', types, args, bad) == 1
+    assert size.value == 7
+    assert _call('shared_prefix_kernel', 'mt_paged_shared_workspace_bytes', types, args, good) == 0
+    assert size.value > 7
+
+
+def test_attention_refuses_more_than_a_launch_has():
+    for bad, _ in PLANS:
+        assert _call('shared_prefix_kernel', 'mt_paged_shared_attention', [P] * 7 + [I] * 15 + [P, Z], ATTEND,
+                     dict(bad, size=1 << 60)) == 1
 
 
 def test_workspace_grows_with_the_batch():

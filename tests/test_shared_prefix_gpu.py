@@ -2,6 +2,7 @@
 through a slot map, one-token decode and ragged attention (include/mt_shared.h),
 and a run of them together. Tolerances are in tests/tolerances.py."""
 import ctypes as ct
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -350,6 +351,65 @@ def test_attention_of_one_token_each_agrees_with_decode(dtype):
     assert_attention_close(one, two, dtype, ref_rounded=True)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('dim', [64, 128, 16])
+def test_attention_of_many_requests_most_of_few_tokens(dtype, dim):
+    # a table far wider than most contexts: the workgroups look up their items
+    b = 300
+    new = [(i * 7) % 4 for i in range(b)]
+    lengths = [(i * 37) % 60 for i in range(b)]
+    new[5], new[290], lengths[17], new[17], lengths[33] = 300, 33, 4075, 9, -1
+    case = SharedCase(30, prefix=50, lengths=lengths, new=new, heads=8, dim=dim, page_size=8, dtype=dtype, columns=513, pps=64,
+                      appended=True, behind=3)
+    case.check_attend()
+    case.check_attend(max_tokens=case.rows)
+
+
+@pytest.mark.parametrize('cu', [[0, 3, 2, 9], [-4, 3, 8, 400], [5, 5, 5, 5], [2 ** 31 - 1, 0, -2 ** 31, 9]])
+def test_attention_wild_offsets_stay_in_bounds_with_a_wide_table(cu):
+    case = SharedCase(31, prefix=40, lengths=[5, 6, 7], new=[3, 3, 3], heads=12, dtype='float16', appended=True, behind=2,
+                      page_size=32, columns=8192)
+    case.dev_cu.upload(np.array(cu, np.int32))
+    case.dev_lengths.upload(np.array([2 ** 31 - 1, 6, -2 ** 31], np.int32))
+    case.attend(max_tokens=9)
+    runtime().synchronize()
+    assert np.array_equal(case.pool_image().view(np.uint8), case.image.view(np.uint8))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('dim', [128, 80])
+def test_attention_many_rows_of_wide_heads(dtype, dim):
+    case = SharedCase(32, prefix=901, lengths=[0, 100, 31, 0], new=[170, 1, 60, 90], heads=3, dim=dim, dtype=dtype, pps=32,
+                      appended=True)
+    case.check_attend()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_prefix_shares_that_cross_tiles(dtype):
+    # 24 (head, tile) of 25 units, three units a workgroup: pieces end in one tile and
+    # start the next
+    case = SharedCase(33, prefix=25 * 128 - 5, lengths=[(5 * i) % 19 for i in range(300)], new=[1] * 300, heads=12, dim=32,
+                      dtype=dtype, pps=256)
+    case.check_decode()
+
+
+@pytest.mark.parametrize('page', [8, 32])
+def test_prefix_pieces_of_the_most_pages(page):
+    case = SharedCase(34, prefix=16384 + 3, lengths=[i % 5 for i in range(260)], new=[1] * 260, heads=32, dim=8,
+                      dtype='float16', page_size=page, pps=512)
+    case.clear()
+    case.decode()
+    got, image = case.result(), case.image.copy()
+    case.append(image)
+    for head in (0, 13, 31):
+        k0, v0 = po.image_gather(image, CODES['float16'], case.prefix_table, len(case.prefix_table), 0, head, case.prefix)
+        for r in (0, 7, 255, 256, 259):
+            k1, v1 = po.image_gather(image, CODES['float16'], case.table[r], case.columns, 0, head, int(case.lengths[r]) + 1)
+            q = po.decode(case.block(0), CODES['float16']).reshape(260, 32, 8)[r, head]
+            ref = po.attention_fp64(q, np.concatenate([k0, k1]), np.concatenate([v0, v1]))
+            assert_attention_close(got[r, head], ref, 'float16', context=f'{head} {r}')
+
+
 # ------------------------------------------------------------ as one uses ---
 def test_calls_repeat_bit_for_bit():
     for dtype in TYPES:
@@ -401,6 +461,29 @@ def test_captured_calls_replay(kind):
             assert_attention_close(case.result(), case.reference(image), 'float16')
     for graph in graphs:
         assert lib.mt_graph_destroy(graph) == 0
+
+
+def test_two_host_threads_at_once():
+    # a stream and a workspace for each
+    cases = [SharedCase(40 + i, prefix=700 + i, lengths=[(37 * r) % 140 for r in range(50)], new=[1] * 50, dtype='bfloat16',
+                        pps=16) for i in range(2)]
+    images = [case.image.copy() for case in cases]
+    for case, image in zip(cases, images):
+        case.append(image)
+
+    def steps(case):
+        outs = []
+        for _ in range(20):
+            case.clear()
+            case.decode()
+            outs.append(case.raw())
+        return outs
+    with ThreadPoolExecutor(2) as pool:
+        both = list(pool.map(steps, cases))
+    for case, image, outs in zip(cases, images, both):
+        for out in outs[1:]:
+            assert np.array_equal(out.view(np.uint8), outs[0].view(np.uint8))
+        assert_attention_close(po.decode(outs[0], CODES['bfloat16']).reshape(outs[0].shape), case.reference(image), 'bfloat16')
 
 
 @pytest.mark.parametrize('dtype,page', [('float32', 16), ('float16', 8), ('bfloat16', 32)])
