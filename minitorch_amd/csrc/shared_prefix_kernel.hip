@@ -11,7 +11,10 @@ using namespace mt;
 namespace {
 
 // ---------------------------------------------------------------------------
-// K/V rows to their pages through a slot map. VEC moves 16 bytes per thread.
+// K/V rows to their pages through a slot map. VEC moves 16 bytes of K and of V per
+// thread, neighbours side by side in the row and, for a head's columns, in the page. Bound
+// by memory: 5001 rows of 25 heads of 64 in bf16 (64 MB moved) 11.6 us, 5.5 TB/s, as fast
+// as a large copy; one launch's latency for few rows (64 rows of 12 heads 2.7 us).
 struct SlotArgs {
   const void* k;
   const void* v;
@@ -1072,7 +1075,10 @@ void shared_kernel(SharedArgs a, Plan p) {
 // cores a key that a query does not attend has weight 0, and 0 * Inf or 0 * NaN of
 // its V is NaN, and so is the 0 * Inf of a weight's low part.
 constexpr int kMergeThreads = 256;
-constexpr int kManyPieces = 8;  // from here on several groups of lanes share a (row, head)
+// From this many pieces on several groups of lanes share a (row, head): 8 requests behind
+// 8192 tokens (32 pieces) 15.8 us with it, 18.7 without; 16 prompts of fp32 (3) 41 without,
+// 44 with it. Between 4 and 16 it makes no difference.
+constexpr int kManyPieces = 8;
 
 // Pieces joined so far: four dims of the accumulators, maximum, denominator.
 struct Joined {
@@ -1207,9 +1213,15 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
   Plan p{};
   p.waves = waves;
   // Prefix tiles: the queries' groups of 32 over tiles of 1, 2, 4 or 8 groups,
-  // where a tile costs its groups and about one more.
+  // where a tile costs its groups and about one more (us in tiles of 1, 2, 4, 8: 64
+  // requests behind 2048 tokens 20.6, 16.7, 17.7, 17.9; 160 rows behind 2048 23.1,
+  // 22.0, 20.7, 19.6). Beside streams of own keys two tiles of 4 do as well as a full one of
+  // 8 or better (256 requests behind 16001 tokens 68 and 74, 400 behind 1000 154 and 160,
+  // 512 of contexts up to 8192 behind 8192 323 and 319), but not those of 240 (47 and 45)
+  // nor prompts' (8 of 300-500 behind 8000 213 and 179).
   int64_t best = INT64_MAX;
-  for (int qt = 1; qt <= waves; qt *= 2) {
+  const int most = decode && row_bytes == 128 && rows >= 256 ? 4 : waves;
+  for (int qt = 1; qt <= most; qt *= 2) {
     const int64_t cost = ceil_div(rows, 32 * qt) * (qt + 1);
     if (cost <= best) { best = cost; p.qt = qt; }
   }
@@ -1252,6 +1264,9 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
                                                : (units - 2) / p.item_units + 2);
   }
   if (decode) {
+    // More waves for a (request, head) where there are few of them: us with 2, 4 and 8
+    // waves, 64 x 12 17.2, 16.8, 20.4; 128 x 16 48, 45, 56; 256 x 16 77.6, 83, 97;
+    // 512 x 25 322, 340, 431.
     const int64_t resident = int64_t(slots) * waves;
     p.item_waves = bh * 8 <= resident ? 8 : bh * 4 <= 2 * resident ? 4 : 2;
     p.item_waves = std::min(p.item_waves, waves);
