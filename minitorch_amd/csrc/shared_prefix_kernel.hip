@@ -355,7 +355,7 @@ struct Tile {
 // kernels'; fp16's are taken 2^kHalfShift larger, whose low parts would
 // otherwise end at 2^-24. The exponentials' reference moves when a score exceeds
 // it by kRescale only.
-template <int DT, int DP, int W>
+template <int DT, int DP, int W, Rows FULL>
 __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, int head, char* s_raw,
                                             typename Elem<DT>::T const** s_page, uint64_t* s_slabs, int* s_missing) {
   using T = typename Elem<DT>::T;
@@ -364,7 +364,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
   constexpr float kShift = DT == kF16 ? kHalfShift : 0.f;
   constexpr int CH = DP == 64 ? 4 : 2;  // chains of an fp32 block's sums
   const Geometry& g = a.g;
-  const int dim = g.dim, chunks = dim / EC;
+  const int dim = FULL == kRowsFull ? DP : g.dim, chunks = dim / EC;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // keeps this tile's terms out of the registers of the tiles before
   const int lane = tid & (kWave - 1);
@@ -374,15 +374,21 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
   const int grp = lane >> 5, col = lane & 31;
   const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)s_raw));
 
-  // B operand of S^T: 16-bit types dims [16 s + 8 grp, + 8) of the lane's query,
-  // fp32 dims [DP / 2 * grp, + DP / 2).
+  // B operand of S^T: chunks 2 s + grp of the lane's query. Products with nothing but
+  // padding are left out for fp32 rows of up to 64, whose products are slow (110 requests
+  // x 25 heads of 32 behind 6697 tokens: 55 us instead of 74); elsewhere the branches cost
+  // more than they save (10 x 5 tokens x 12 heads of 72 in fp16 behind 1272: 19.3 and 17.6).
+  constexpr bool TRIM = DT == kF32 && DP == 64 && FULL == kRowsPadded;
+  const int s_end = (chunks + 1) / 2, d_end = (dim + 31) / 32;
+  auto in_s = [&](int s) { return !TRIM || s < s_end; };
+  auto in_d = [&](int d) { return !TRIM || d < d_end; };
   const int q0 = qt * 32, qi = q0 + col;
   const bool live = q0 < t.nq;
   const T* qrow = static_cast<const T*>(t.q) + (qi < t.nq ? qi : 0) * a.q_r;
   u32x4 qv[QW];
 #pragma unroll
   for (int s = 0; s < QW; ++s) {
-    const int p = DT == kF32 ? CPR / 2 * grp + s : 2 * s + grp;
+    const int p = 2 * s + grp;
     qv[s] = *global_view(reinterpret_cast<const u32x4*>(p < chunks ? qrow + p * EC : reinterpret_cast<const T*>(g_fill + 4)));
   }
 
@@ -408,7 +414,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     if (!page) *s_missing = 1;
   }
   __syncthreads();
-  const bool plain = !*s_missing && chunks == CPR;
+  const bool plain = FULL == kRowsFull && !*s_missing;
 
   // Keys [k, k + kHalf) into half `h`. Keys past the end are zero; a missing
   // page is NaN in K (its scores are NaN) and zero in V.
@@ -492,7 +498,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
   };
   // K's operand s of the block of 32 keys at s_k, for S^T.
   auto read_k = [&](const T* s_k, int s) {
-    const int p = DT == kF32 ? CPR / 2 * grp + s : 2 * s + grp;
+    const int p = 2 * s + grp;
     return *reinterpret_cast<const u32x4*>(s_k + col * DP + S::kpos(col, p) * EC);
   };
   // O^T += V^T P^T for 16-bit types, 16 keys a step: slot j < 4 of a lane holds key
@@ -512,6 +518,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
       u32x4 vt[DT32];
 #pragma unroll
       for (int d = 0; d < DT32; ++d) {
+        if (!in_d(d)) break;
         const int rr = 4 * grp + (t16 >> 2);
         const int p = 4 * d + ((lane >> 4) & 1) * 2 + ((t16 & 3) >> 1);
         const T* v_at = s_v + (16 * s + rr) * DP + S::vpos(rr, p) * 8 + (t16 & 1) * 4;
@@ -520,9 +527,11 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
       }
       // (no product waits for the one before it)
 #pragma unroll
-      for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], hi, o[d]);
+      for (int d = 0; d < DT32; ++d)
+        if (in_d(d)) o[d] = mfma32<DT>(vt[d], hi, o[d]);
 #pragma unroll
-      for (int d = 0; d < DT32; ++d) o[d] = mfma32<DT>(vt[d], lo, o[d]);
+      for (int d = 0; d < DT32; ++d)
+        if (in_d(d)) o[d] = mfma32<DT>(vt[d], lo, o[d]);
     }
   };
   auto keys_at = [&](int h, int at) { return reinterpret_cast<const T*>(s_raw + h * 2 * S::kPlane) + at * DP; };
@@ -544,6 +553,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
         for (int i = 0; i < 16; ++i) part[j][i] = 0.f;
 #pragma unroll
       for (int s = 0; s < QW; ++s) {
+        if (!in_s(s)) break;
         const u32x4 kf = read_k(s_k, s);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -555,7 +565,8 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
       for (int i = 0; i < 16; ++i) sc[i] = (part[0][i] + part[1][i]) + (CH == 4 ? part[CH - 2][i] + part[CH - 1][i] : 0.f);
     } else {
 #pragma unroll
-      for (int s = 0; s < QW; ++s) sc = mfma32<DT>(read_k(s_k, s), qv[s], sc);
+      for (int s = 0; s < QW; ++s)
+        if (in_s(s)) sc = mfma32<DT>(read_k(s_k, s), qv[s], sc);
     }
     // limits, only for blocks that reach past one (a wave-uniform test)
     if (base + 31 > t.limit + q0 || base + 32 > t.k1) {
@@ -572,6 +583,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
       // a block's sums start at zero, in chains, and are added to the running ones
 #pragma unroll
       for (int d = 0; d < DT32; ++d) {
+        if (!in_d(d)) break;
         floatx16 ob[CH];
 #pragma unroll
         for (int j = 0; j < CH; ++j)
@@ -601,6 +613,7 @@ __device__ __forceinline__ void attend_tile(const SharedArgs& a, const Tile& t, 
     for (int i = 0; i < 16; ++i) s0[i] = s1[i] = 0.f;
 #pragma unroll
     for (int s = 0; s < QW; ++s) {
+      if (!in_s(s)) break;
       s0 = mfma32<DT>(read_k(k0, s), qv[s], s0);
       s1 = mfma32<DT>(read_k(k1, s), qv[s], s1);
     }
@@ -921,7 +934,7 @@ __device__ __forceinline__ void stream_more(const SharedArgs& a, const Plan& p, 
 // of 8192: 366 us, with a workgroup for each of 245000 bounds 1230.
 constexpr int kListed = 256;
 
-template <int DT, int DP, int W>
+template <int DT, int DP, int W, Rows FULL>
 __device__ __forceinline__ void own_item(const SharedArgs& a, const Plan& p, int r, const Request& rq, int tile, int split,
                                          int head, char* s_raw, typename Elem<DT>::T const** s_page, uint64_t* s_slabs,
                                          int* s_missing) {
@@ -945,10 +958,10 @@ __device__ __forceinline__ void own_item(const SharedArgs& a, const Plan& p, int
   t.k1 = int(min(end, k0 + p.split_keys));
   t.limit = int64_t(rq.length) + q0;
   t.part = part_of<DP>(a, p, p.pieces + split, head, row);
-  attend_tile<DT, DP, W>(a, t, head, s_raw, s_page, s_slabs, s_missing);
+  attend_tile<DT, DP, W, FULL>(a, t, head, s_raw, s_page, s_slabs, s_missing);
 }
 
-template <int DT, int DP, int W>
+template <int DT, int DP, int W, Rows FULL>
 __device__ __forceinline__ void listed_items(const SharedArgs& a, const Plan& p, int block, char* s_raw,
                                              typename Elem<DT>::T const** s_page, uint64_t* s_slabs, int* s_missing,
                                              int* s_count) {
@@ -989,7 +1002,7 @@ __device__ __forceinline__ void listed_items(const SharedArgs& a, const Plan& p,
       const int item = x - (i ? __builtin_amdgcn_readfirstlane(s_count[i - 1]) : 0);
       const Request rq = request_of(a, r0 + i);
       const int tiles = max(1, (rq.tokens + tq - 1) / tq), split = item / tiles;
-      own_item<DT, DP, W>(a, p, r0 + i, rq, item - split * tiles, split, head, s_raw, s_page, s_slabs, s_missing);
+      own_item<DT, DP, W, FULL>(a, p, r0 + i, rq, item - split * tiles, split, head, s_raw, s_page, s_slabs, s_missing);
       __syncthreads();  // the LDS is done with
     }
     next -= all;
@@ -1035,7 +1048,7 @@ void shared_kernel(SharedArgs a, Plan p) {
       t.k1 = min(a.prefix, (unit + n) * p.prefix_unit);
       t.limit = INT_MAX;
       t.part = part_of<DP>(a, p, index - __builtin_amdgcn_readfirstlane(first_item(p, head_tile)), head, row);
-      attend_tile<DT, DP, W>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
+      attend_tile<DT, DP, W, FULL>(a, t, head, s_raw, s_page, s_slabs, &s_missing);
       at += n;
       if (at < end) __syncthreads();  // the LDS is done with
     }
@@ -1056,14 +1069,15 @@ void shared_kernel(SharedArgs a, Plan p) {
     stream_item<DT, DP, W, FULL>(a, p, on, row, on ? int(item - int64_t(row) * g.heads) : 0, -1,
                               reinterpret_cast<float*>(s_raw), s_slabs, slabs_there);
   } else if constexpr (OWN == kOwnTiles) {
-    // (split, request, tile, head)
+    // (split, tile, request, head), the last tiles, which attend the most keys, first (16
+    // prompts of 453 x 16 heads fp32: 171 us, 204 in order)
     const int i = index / g.heads, head = index - i * g.heads;
-    const int rt = i / p.own_tiles, tile = i - rt * p.own_tiles;
-    const int split = rt / a.b, r = rt - split * a.b;
-    own_item<DT, DP, W>(a, p, r, request_of(a, r), tile, split, head, s_raw, s_page, s_slabs, &s_missing);
+    const int st = i / a.b, r = i - st * a.b;
+    const int split = st / p.own_tiles, tile = p.own_tiles - 1 - (st - split * p.own_tiles);
+    own_item<DT, DP, W, FULL>(a, p, r, request_of(a, r), tile, split, head, s_raw, s_page, s_slabs, &s_missing);
   } else {
     __shared__ int s_count[kListed + kListed / kWave];
-    listed_items<DT, DP, W>(a, p, index, s_raw, s_page, s_slabs, &s_missing, s_count);
+    listed_items<DT, DP, W, FULL>(a, p, index, s_raw, s_page, s_slabs, &s_missing, s_count);
   }
 }
 
@@ -1225,6 +1239,9 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
     const int64_t cost = ceil_div(rows, 32 * qt) * (qt + 1);
     if (cost <= best) { best = cost; p.qt = qt; }
   }
+  // Smaller ones where the prefix is too short for an item on each compute unit (decode 257 x
+  // 12 behind 199 tokens 14.6 us, 18.6 without; prompts gain and lose by it).
+  while (decode && p.qt > 1 && ceil_div(rows, 32 * p.qt) * h * ceil_div(prefix, 64) < cus) p.qt /= 2;
   p.tiles = int(ceil_div(rows, 32 * p.qt));
   if (prefix > 0) {
     // Units of a staged half. One item a compute unit, which leaves half of its
@@ -1235,11 +1252,16 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
     // requests of 1-20 tokens x 12 behind 4096 50, 42 and 49; one decode row x 12
     // behind 32000 40, 29 and 27; 24 prompts x 16 heads of 128 behind 8100 (eight waves)
     // 358, 378 and 390, with three quarters 356.
+    // Where the own items are few (they fit beside each other), prefix items take every
+    // place too: 16 prompts of 256-512 behind 2048 105 us instead of 120.
     // Pieces of 256 keys at least unless few would be left (4 rows fp32 x 12 heads behind
     // 200: 10.5 in pieces of 64, 13 whole), cut at the tiles' ends where that keeps nine
     // tenths of the items busy, for the fewest pieces.
     const int64_t head_tiles = int64_t(p.tiles) * h;
-    const int64_t want = 2 * p.qt < waves ? slots : slots > cus || dtype == kF32 ? cus : 3 * int64_t(cus) / 4;
+    const int64_t own = decode ? INT64_MAX : bh * ceil_div(max_tokens, 256) * ceil_div(cap + 1, 2048);
+    const int64_t want = 2 * p.qt < waves || (row_bytes == 128 && own <= slots) ? slots
+                         : slots > cus || dtype == kF32                         ? cus
+                                                                                : 3 * int64_t(cus) / 4;
     p.prefix_unit = row_bytes == 128 ? 128 : 64;
     int64_t units = ceil_div(prefix, p.prefix_unit);
     if (head_tiles * ceil_div(prefix, 256) < cus / 4) {
@@ -1270,7 +1292,10 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
     const int64_t resident = int64_t(slots) * waves;
     p.item_waves = bh * 8 <= resident ? 8 : bh * 4 <= 2 * resident ? 4 : 2;
     p.item_waves = std::min(p.item_waves, waves);
-    while (p.item_waves > 1 && (p.item_waves - 1) * 8 >= cap) p.item_waves /= 2;
+    // A wave has eight tokens at least, where there are many rows 64 (512 x 12 behind 4096 and
+    // own contexts up to 64: 38 us with one wave, 41 with two).
+    const int least = bh > resident ? 64 : 8;
+    while (p.item_waves > 1 && (p.item_waves - 1) * least >= cap) p.item_waves /= 2;
     // Splits of 512 tokens: a wave resolves the page of each of its steps into one
     // lane, 64 steps of 8 tokens. Longer ones for tables of more than 64.
     p.split_keys = int(std::min<int64_t>(512 * p.item_waves, std::max<int64_t>(512, ceil_div(cap, 64 * 64) * 64)));
@@ -1306,21 +1331,25 @@ size_t plan_bytes(const Plan& p, int rows, int h, int d) {
 // Rows that the fast path takes: whole 16-byte chunks.
 bool whole_chunks(int d, int dtype) { return d * (dtype == kF32 ? 4 : 2) % 16 == 0; }
 
-template <int DT, int DP, int W>
+template <int DT, int DP, int W, Rows FULL>
 void launch_tiles(const SharedArgs& a, const Plan& p) {
   const int blocks = int(p.prefix_items + p.own_blocks);
-  if (p.listed) shared_kernel<DT, DP, W, kRowsFull, kOwnListed><<<blocks, W * kWave>>>(a, p);
-  else shared_kernel<DT, DP, W, kRowsFull, kOwnTiles><<<blocks, W * kWave>>>(a, p);
+  if (p.listed) shared_kernel<DT, DP, W, FULL, kOwnListed><<<blocks, W * kWave>>>(a, p);
+  else shared_kernel<DT, DP, W, FULL, kOwnTiles><<<blocks, W * kWave>>>(a, p);
+}
+
+template <int DT, int DP, Rows FULL>
+void launch_rows(const SharedArgs& a, const Plan& p) {
+  constexpr int W = shape_waves(DP * elem_bytes<DT>(), false);
+  if (a.k) shared_kernel<DT, DP, W, FULL, kOwnToken><<<int(p.prefix_items + p.more_blocks + p.own_blocks), W * kWave>>>(a, p);
+  else if (p.waves == W) launch_tiles<DT, DP, W, FULL>(a, p);
+  else if constexpr (W == 4 && DT != kF32) launch_tiles<DT, DP, 8, FULL>(a, p);
 }
 
 template <int DT, int DP>
 void launch_fast(const SharedArgs& a, const Plan& p) {
-  constexpr int W = shape_waves(DP * elem_bytes<DT>(), false);
-  const int blocks = int(p.prefix_items + p.more_blocks + p.own_blocks);
-  if (a.k && a.g.dim == DP) shared_kernel<DT, DP, W, kRowsFull, kOwnToken><<<blocks, W * kWave>>>(a, p);
-  else if (a.k) shared_kernel<DT, DP, W, kRowsPadded, kOwnToken><<<blocks, W * kWave>>>(a, p);
-  else if (p.waves == W) launch_tiles<DT, DP, W>(a, p);
-  else if constexpr (W == 4 && DT != kF32) launch_tiles<DT, DP, 8>(a, p);
+  if (a.g.dim == DP) launch_rows<DT, DP, kRowsFull>(a, p);
+  else launch_rows<DT, DP, kRowsPadded>(a, p);
   const int64_t pairs = int64_t(a.rows) * a.g.heads;
   constexpr int LANES = DP / 4;
   if (p.pieces >= kManyPieces) shared_merge_kernel<DT, DP, kWave / LANES><<<int(ceil_div(pairs, kMergeThreads / kWave)), kMergeThreads>>>(a, p);
