@@ -641,7 +641,7 @@ __global__ __launch_bounds__(kThreads) void decode_abort_kernel(Pool p, const in
 // the table that is read (a started page, held before the step) is never one that
 // is written. Bound by latency (lengths, scan, pages, stores; a launch
 // that does nothing takes about 3 us of these): 3.4 us for 64 decode tokens, 3.7
-// for 96 and 32 prompts, 6.0 for 512 prompts (356k tokens, 4.3 MB, 0.9 us at the
+// for 96 and 32 prompts, 6.0 for 512 prompts (265k tokens, 4.3 MB, 0.9 us at the
 // copy rate).
 constexpr int kChunk = 256;
 constexpr int kTableThreads = 256;
@@ -921,7 +921,7 @@ int mt_sched_batch_tables(int* table, int64_t* slots, float* positions, int* cu_
   a.b = b; a.rows = rows; a.page_count = page_count; a.columns = columns; a.prefix = prefix_tokens;
   a.log2_page = page_size == 8 ? 3 : page_size == 16 ? 4 : 5;
   // Shares of a chunk: a token or page a thread, up to three workgroups a compute
-  // unit (512 prompts of 356k tokens: 6.0 us; two 6.4, six 6.0, eight tokens a
+  // unit (512 prompts of 265k tokens: 6.0 us; two 6.4, six 6.0, eight tokens a
   // thread at small steps 3.8 instead of 3.6).
   const int chunks = (b + kChunk - 1) / kChunk;
   const int64_t work = int64_t(rows) + page_count;
