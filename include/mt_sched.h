@@ -146,10 +146,9 @@ int mt_sched_decode_abort(MT_POOL_ARGS, const int* slots, int b, const int* new_
  * negative, or the list is exhausted (whose table entries are -1 as well). A request of negative length is
  * left out: it takes no token and no page, and its row stays. Negative tokens
  * count as none. lengths, tokens and pages are read on the device and may hold
- * anything. 1 <= b <= 65535; rows < 2^24; page_size
- * 8, 16 or 32; page_count 0 needs no list, and
- * 2^30 is the most. One launch on the
- * calling thread's default stream; nothing is allocated. Replaces, for several tokens per request, the host
+ * anything. 1 <= b <= 65535; rows < 2^24; page_size 8, 16 or 32; page_count 0
+ * needs no list, and 2^30 is the most. One launch on the calling thread's default
+ * stream; nothing is allocated. Replaces, for several tokens per request, the host
  * tables of reference PagedDecodeBatch.prepare (minitorch/paged_decode.py:40-54) and
  * PagedKVCache.prepare_append (minitorch/paged_kv_cache.py:171-189). */
 int mt_sched_batch_tables(int* table, int64_t* slots, float* positions, int* cu_tokens, const int* lengths,

@@ -10,12 +10,16 @@
  * a page). Every query attends the whole prefix, then its request's own tokens
  * up to itself. The prefix is read once for many requests' queries (tiles of up
  * to 256), not once per request. A missing page (mt_paged.h) makes every query
- * that attends it NaN; one of the prefix all of them.
+ * that attends it NaN; one of the prefix all of them. Inf and NaN of K and V reach
+ * the queries that attend them and no others (rows beside or behind such values
+ * in V are computed once more one by one, which is slow).
  *
  * Workspace: partial results, of the size that mt_paged_shared_workspace_bytes
  * reports for the same sizes (0: none is needed, and it may be null), 16-byte
  * aligned, with no content to keep between calls; calls that share one must not
- * overlap, nor must replays of graphs captured with it. `out` overlaps no input.
+ * overlap, nor must replays of graphs captured with it. Fewer rows can need more
+ * (their keys are cut more often): one for several sizes takes the largest of theirs.
+ * `out` overlaps no input.
  * Sizes: h <= 65535 / b; rows * h * d, prefix and own tokens of a table together
  * below 2^31; for rows of whole 16-byte chunks also rows * h < 2^26, and at most 2^22
  * pieces of work of one kind (tiles of up to 256 rows x the cuts of the longest
@@ -52,9 +56,10 @@ int mt_paged_shared_workspace_bytes(int rows, int b, int h, int d, int page_size
  * tokens. A request of negative offset is padding: its output row is zero and
  * nothing is written. One past the table's columns has a NaN row and writes
  * nothing. Without a prefix this is mt_paged_decode_batch up to the order of
- * its sums. Two launches at most; nothing is allocated, so that the call can be captured. Requests must not
- * share a page that this call writes. No reference counterpart (the reference reads a shared prefix once per
- * request, src/paged_attention_kernel.cu:121-137). */
+ * its sums. Two launches at most; nothing is allocated, so that the call can be
+ * captured. Requests must not share a page that this call writes. No reference
+ * counterpart (the reference reads a shared prefix once per request,
+ * src/paged_attention_kernel.cu:121-137). */
 int mt_paged_shared_decode(void* out, const void* q, const void* k, const void* v, const uint64_t* slabs,
                            const int* prefix_table, const int* table, const int* offsets, int b, int h, int d,
                            int page_size, int pages_per_slab, int num_slabs, int prefix_tokens, int columns,
@@ -69,9 +74,9 @@ int mt_paged_shared_decode(void* out, const void* q, const void* k, const void* 
  * lengths[r] + i] (lengths: device, own tokens before the new ones; negative:
  * padding, whose rows are zero). max_tokens bounds the new tokens of any one
  * request: rows past it, like those behind the last request's, are not
- * written. 1 <= b <= 65535, max_tokens <= rows. No launch
- * depends on device values, and nothing is allocated, so that the call can be captured.
- * No reference counterpart. */
+ * written. 1 <= b <= 65535, max_tokens <= rows. No launch depends on device
+ * values, and nothing is allocated, so that the call can be captured. No
+ * reference counterpart. */
 int mt_paged_shared_attention(void* out, const void* q, const uint64_t* slabs, const int* prefix_table,
                               const int* table, const int* lengths, const int* cu_tokens, int b, int rows,
                               int max_tokens, int h, int d, int page_size, int pages_per_slab, int num_slabs,
