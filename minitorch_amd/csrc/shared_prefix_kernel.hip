@@ -1246,7 +1246,7 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
   int64_t best = INT64_MAX;
   const int most = decode && row_bytes == 128 && rows >= 256 ? 4 : waves;
   for (int qt = 1; qt <= most; qt *= 2) {
-    const int64_t cost = ceil_div(rows, 32 * qt) * (qt + 1);
+    const int64_t cost = ceil_div(rows, 32 * qt) * ((dtype == kF32 ? 3 * qt : qt) + 1);
     if (cost <= best) { best = cost; p.qt = qt; }
   }
   // Smaller ones where the prefix is too short for an item on each compute unit (decode 257 x
