@@ -1243,6 +1243,9 @@ Plan make_plan(int rows, int b, int h, int d, int page_size, int prefix, int col
   // 8 or better (256 requests behind 16001 tokens 68 and 74, 400 behind 1000 154 and 160,
   // 512 of contexts up to 8192 behind 8192 323 and 319), but not those of 240 (47 and 45)
   // nor prompts' (8 of 300-500 behind 8000 213 and 179).
+  // fp32 products are slow, so that waves without queries cost more there: groups count three
+  // times (with that and without, 6 prompts of 9-37 x 25 behind 3546 54 and 65, 75 requests x
+  // 25 of 32 behind 12684 83 and 90, 66 x 12 behind 4000 36 and 33).
   int64_t best = INT64_MAX;
   const int most = decode && row_bytes == 128 && rows >= 256 ? 4 : waves;
   for (int qt = 1; qt <= most; qt *= 2) {
